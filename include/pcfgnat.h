@@ -54,6 +54,7 @@ extern "C" {
 
 #define PCFGNAT_DTYPE_F32 0
 #define PCFGNAT_DTYPE_F16 1
+#define PCFGNAT_DTYPE_BF16 2 /* token_logprobs, embed and clip_grad_norm entry points only */
 
 int pcfgnat_version(void);
 const char *pcfgnat_error_string(int code);
@@ -422,6 +423,58 @@ int pcfgnat_plan_real_rows(const int64_t *host_lengths, int b0, int b1, int L, i
  * change until the kernel has run. */
 int pcfgnat_stage_inputs(const void *hidden_src, void *hidden_dst, int row_bytes, const float *links_src,
                          float *links_dst, const int64_t *output_length, int B, int L, int max_left, void *stream);
+
+/* ---- The vocabulary table at both ends, and the step behind the backward pass.  No counterpart among the reference's
+ * operators: its model looks tokens up with torch's embedding and its trainer clips with torch's operators. ---- */
+
+/* Log probabilities of given tokens from materialised logits, with entropy and best alternatives.
+ * Row r of the logits (PCFGNAT_DTYPE_*, V numbers in a row) begins (r / rows_inner) * stride_outer + (r % rows_inner) *
+ * stride_inner numbers behind `logits`.  tokens [rows]; logprob [rows]; optional (NULL: not wanted) entropy [rows] in nats;
+ * top_logprob and top_index [rows][top] (0 <= top <= PCFGNAT_MAX_TOP), values falling, equal ones by rising index; kept
+ * [rows][2] for the backward call.  Everything is formed in float32.
+ * Rows whose token is ignore_index (with has_ignore) are left out: 0, 0, (0, -1).  Entries of -inf have no probability and
+ * are no alternatives: where there are fewer than `top` others, the rest is (-inf, -1).  A row of nothing but -inf gives
+ * logprob -inf and entropy 0, one with NaN or +inf NaN and indices -1.  A token outside [0, V) gives logprob NaN and
+ * PCFGNAT_STATUS_BAD_INDEX. */
+#define PCFGNAT_MAX_TOP 32
+int pcfgnat_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t rows_inner, int64_t stride_outer,
+                           int64_t stride_inner, int V, const int64_t *tokens, int has_ignore, int64_t ignore_index, int top,
+                           float *logprob, float *entropy, float *top_logprob, int64_t *top_index, float *kept, int *status,
+                           void *stream);
+/* The gradient of the logits, in their type, every cell of d_logits [rows][pitch] up to V (pitch >= V; what lies behind V stays
+ * as it is).  grad_logprob [rows], grad_entropy [rows] (with the forward's entropy) and grad_top [rows][top] (with its
+ * top_index) may each be NULL.  Rows that were left out, and rows of nothing but -inf, get zeros; a row whose token is out of
+ * range gets NaN when grad_logprob is given. */
+int pcfgnat_token_logprobs_backward(const void *logits, int dtype, int64_t rows, int64_t rows_inner, int64_t stride_outer,
+                                    int64_t stride_inner, int V, const int64_t *tokens, int has_ignore, int64_t ignore_index,
+                                    int top, const float *kept, const float *entropy, const int64_t *top_index,
+                                    const float *grad_logprob, const float *grad_entropy, const float *grad_top, void *d_logits,
+                                    int64_t pitch, int *status, void *stream);
+
+/* out [n][H] = scale * weight[tokens[i]], formed in float32 and rounded to the table's type (PCFGNAT_DTYPE_*); the table's
+ * rows lie weight_stride numbers apart.  A token outside [0, V) gives a row of NaN and PCFGNAT_STATUS_BAD_INDEX. */
+int pcfgnat_embed(const void *weight, int dtype, int64_t weight_stride, int64_t V, int H, const int64_t *tokens, int64_t n,
+                  float scale, void *out, int *status, void *stream);
+/* The table's gradient: row v of d_weight [V] (grad_stride, d_stride: numbers between rows) = scale * the sum of grad_out's rows
+ * whose token is v, in float32 and in an order that the tokens alone decide.  Tokens equal to padding_idx (with has_padding) and
+ * tokens out of range (flagged) count for nothing.  d_dtype is PCFGNAT_DTYPE_F32 or grad_out's dtype.  accumulate: added onto the
+ * rows that occur, the others stay as they are; otherwise every row is written.  n < 2^31. */
+size_t pcfgnat_embed_backward_workspace_bytes(int64_t n, int64_t V, int H);
+int pcfgnat_embed_backward(const void *grad_out, int dtype, int64_t grad_stride, const int64_t *tokens, int64_t n, int64_t V,
+                           int H, float scale, int has_padding, int64_t padding_idx, void *d_weight, int d_dtype,
+                           int64_t d_stride, int accumulate, void *workspace, size_t workspace_bytes, int *status,
+                           void *stream);
+
+/* Global norm of n gradient tensors and clipping: *norm (device) = |grad_scale| sqrt(sum of all squares), and with
+ * c = min(1, max_norm / (norm + 1e-6))  dst[i] = c * grad_scale * src[i], the products formed in float32.  dst[i] is src[i]
+ * itself (left alone where c * grad_scale is 1) or memory that overlaps no other tensor (PCFGNAT_ERR_INVALID_ARGUMENT
+ * otherwise); dst_dtype[i] is src_dtype[i] or PCFGNAT_DTYPE_F32.  The arrays are host memory and are read before the call
+ * returns; sums are held in float64 and do not depend on timing.  A norm of NaN makes every output NaN; an infinite one makes them
+ * 0, and NaN where the gradient is infinite or NaN. */
+size_t pcfgnat_clip_grad_norm_workspace_bytes(int n);
+int pcfgnat_clip_grad_norm(int n, const void *const *src, const int *src_dtype, void *const *dst, const int *dst_dtype,
+                           const int64_t *size, float max_norm, float grad_scale, void *workspace, size_t workspace_bytes,
+                           float *norm, void *stream);
 
 #ifdef __cplusplus
 }

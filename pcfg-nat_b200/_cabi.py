@@ -54,6 +54,15 @@ SIGNATURES = {
     "pcfgnat_loss_stats_exchange": (c_int, [c_void] * 2 + [c_int] + [c_void] + [c_int] * 2 + [c_void] * 3),
     "pcfgnat_glance_select": (c_int, [c_void] * 7 + [c_int, ctypes.c_float] + [c_int] * 3 + [c_void] * 7),
     "pcfgnat_force_emit": (c_int, [c_void] * 3 + [c_int] * 3 + [c_void] * 2),
+    "pcfgnat_token_logprobs": (c_int, [c_void, c_int] + [c_i64] * 4 + [c_int, c_void, c_int, c_i64, c_int] + [c_void] * 7),
+    "pcfgnat_token_logprobs_backward": (c_int, [c_void, c_int] + [c_i64] * 4 + [c_int, c_void, c_int, c_i64, c_int] + [c_void] * 7 +
+                                        [c_i64] + [c_void] * 2),
+    "pcfgnat_embed": (c_int, [c_void, c_int, c_i64, c_i64, c_int, c_void, c_i64, ctypes.c_float] + [c_void] * 3),
+    "pcfgnat_embed_backward_workspace_bytes": (c_size, [c_i64, c_i64, c_int]),
+    "pcfgnat_embed_backward": (c_int, [c_void, c_int, c_i64, c_void, c_i64, c_i64, c_int, ctypes.c_float, c_int, c_i64, c_void, c_int,
+                                       c_i64, c_int, c_void, c_size, c_void, c_void]),
+    "pcfgnat_clip_grad_norm_workspace_bytes": (c_size, [c_int]),
+    "pcfgnat_clip_grad_norm": (c_int, [c_int] + [c_void] * 5 + [ctypes.c_float] * 2 + [c_void, c_size] + [c_void] * 2),
     "pcfgnat_force_emit_grad": (c_int, [c_void] * 2 + [c_int] * 3 + [c_void] * 2),
 }
 

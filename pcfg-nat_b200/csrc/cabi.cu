@@ -678,4 +678,99 @@ int pcfgnat_links_from_scores(const float *ac, const float *bc, const float *qm,
                                     slot_of, nodes, M, B, L, heads, head_dim, links, static_cast<cudaStream_t>(stream));
 }
 
+int pcfgnat_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t rows_inner, int64_t stride_outer,
+                           int64_t stride_inner, int V, const int64_t *tokens, int has_ignore, int64_t ignore_index, int top,
+                           float *logprob, float *entropy, float *top_logprob, int64_t *top_index, float *kept, int *status,
+                           void *stream) {
+    PCFGNAT_API_RANGE();
+    if (rows < 0 || rows_inner < 1 || V < 1 || top < 0 || top > PCFGNAT_MAX_TOP) return PCFGNAT_ERR_INVALID_ARGUMENT;
+    if (rows && (!logits || !tokens || !logprob || (top && (!top_logprob || !top_index)))) return PCFGNAT_ERR_INVALID_ARGUMENT;
+    if (rows > INT32_MAX) return PCFGNAT_ERR_TOO_LARGE;
+    return launch_token_logprobs(logits, dtype, rows, rows_inner, stride_outer, stride_inner, V, tokens, has_ignore != 0, ignore_index,
+                                 top, logprob, entropy, top_logprob, top_index, kept, status, static_cast<cudaStream_t>(stream));
+}
+
+int pcfgnat_token_logprobs_backward(const void *logits, int dtype, int64_t rows, int64_t rows_inner, int64_t stride_outer,
+                                    int64_t stride_inner, int V, const int64_t *tokens, int has_ignore, int64_t ignore_index,
+                                    int top, const float *kept, const float *entropy, const int64_t *top_index,
+                                    const float *grad_logprob, const float *grad_entropy, const float *grad_top, void *d_logits,
+                                    int64_t pitch, int *status, void *stream) {
+    PCFGNAT_API_RANGE();
+    if (rows < 0 || rows_inner < 1 || V < 1 || top < 0 || top > PCFGNAT_MAX_TOP || pitch < V) return PCFGNAT_ERR_INVALID_ARGUMENT;
+    if (rows && (!logits || !tokens || !kept || !d_logits || (grad_entropy && !entropy) || (grad_top && top && !top_index)))
+        return PCFGNAT_ERR_INVALID_ARGUMENT;
+    if (rows > INT32_MAX) return PCFGNAT_ERR_TOO_LARGE;
+    return launch_token_logprobs_grad(logits, dtype, rows, rows_inner, stride_outer, stride_inner, V, tokens, has_ignore != 0,
+                                      ignore_index, top, kept, entropy, top_index, grad_logprob, grad_entropy, grad_top, d_logits,
+                                      pitch, status, static_cast<cudaStream_t>(stream));
+}
+
+int pcfgnat_embed(const void *weight, int dtype, int64_t weight_stride, int64_t V, int H, const int64_t *tokens, int64_t n,
+                  float scale, void *out, int *status, void *stream) {
+    PCFGNAT_API_RANGE();
+    if (n < 0 || V < 1 || H < 1 || weight_stride < 0) return PCFGNAT_ERR_INVALID_ARGUMENT;
+    if (n && (!weight || !tokens || !out)) return PCFGNAT_ERR_INVALID_ARGUMENT;
+    return launch_embed(weight, dtype, weight_stride, V, H, tokens, n, scale, out, status, static_cast<cudaStream_t>(stream));
+}
+
+size_t pcfgnat_embed_backward_workspace_bytes(int64_t n, int64_t V, int H) {
+    if (n < 0 || V < 1 || H < 1) return 0;
+    return embed_workspace_bytes(n, H);
+}
+
+int pcfgnat_embed_backward(const void *grad_out, int dtype, int64_t grad_stride, const int64_t *tokens, int64_t n, int64_t V,
+                           int H, float scale, int has_padding, int64_t padding_idx, void *d_weight, int d_dtype,
+                           int64_t d_stride, int accumulate, void *workspace, size_t workspace_bytes, int *status,
+                           void *stream) {
+    PCFGNAT_API_RANGE();
+    if (n < 0 || V < 1 || H < 1 || grad_stride < 0 || d_stride < H) return PCFGNAT_ERR_INVALID_ARGUMENT;
+    if (!d_weight || !workspace || (n && (!grad_out || !tokens))) return PCFGNAT_ERR_INVALID_ARGUMENT;
+    if (dtype < 0 || dtype > PCFGNAT_DTYPE_BF16 || (d_dtype != PCFGNAT_DTYPE_F32 && d_dtype != dtype)) return PCFGNAT_ERR_UNSUPPORTED;
+    if (n > INT32_MAX || V > INT32_MAX || H > (1 << 28)) return PCFGNAT_ERR_TOO_LARGE;
+    if (workspace_bytes < embed_workspace_bytes(n, H)) return PCFGNAT_ERR_WORKSPACE;
+    return launch_embed_backward(grad_out, dtype, grad_stride, tokens, n, V, H, scale, has_padding != 0, padding_idx, d_weight, d_dtype,
+                                 d_stride, accumulate != 0, workspace, status, static_cast<cudaStream_t>(stream));
+}
+
+size_t pcfgnat_clip_grad_norm_workspace_bytes(int n) {
+    return n < 0 ? 0 : sizeof(double) * (size_t)(n > 0 ? clip_grad_norm_sums(n) : 1);
+}
+
+int pcfgnat_clip_grad_norm(int n, const void *const *src, const int *src_dtype, void *const *dst, const int *dst_dtype,
+                           const int64_t *size, float max_norm, float grad_scale, void *workspace, size_t workspace_bytes,
+                           float *norm, void *stream) {
+    PCFGNAT_API_RANGE();
+    if (n < 0 || !norm || !workspace || !(max_norm >= 0.f) || (n && (!src || !src_dtype || !dst || !dst_dtype || !size)))
+        return PCFGNAT_ERR_INVALID_ARGUMENT;
+    struct Span {
+        uintptr_t begin, end;
+        int tensor;
+    };
+    try {  // every output overlaps nothing but its own source, exactly
+        std::vector<Span> spans;
+        spans.reserve(2 * (size_t)n);
+        for (int i = 0; i < n; i++) {
+            if (size[i] < 0 || (size[i] && (!src[i] || !dst[i]))) return PCFGNAT_ERR_INVALID_ARGUMENT;
+            if (src_dtype[i] < 0 || src_dtype[i] > PCFGNAT_DTYPE_BF16 ||
+                (dst_dtype[i] != src_dtype[i] && dst_dtype[i] != PCFGNAT_DTYPE_F32) || (size[i] && dst[i] == src[i] && dst_dtype[i] != src_dtype[i]))
+                return PCFGNAT_ERR_UNSUPPORTED;
+            if (size[i] == 0) continue;
+            const auto span = [&](const void *p, int dtype) {
+                const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+                spans.push_back({at, at + (uintptr_t)size[i] * (dtype == PCFGNAT_DTYPE_F32 ? 4 : 2), i});
+            };
+            span(dst[i], dst_dtype[i]);
+            if (src[i] != dst[i]) span(src[i], src_dtype[i]);
+        }
+        std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.begin < b.begin; });
+        for (size_t i = 0; i + 1 < spans.size(); i++)
+            if (spans[i + 1].begin < spans[i].end) return PCFGNAT_ERR_INVALID_ARGUMENT;
+    } catch (...) {
+        return PCFGNAT_ERR_TOO_LARGE;
+    }
+    if (workspace_bytes < pcfgnat_clip_grad_norm_workspace_bytes(n)) return PCFGNAT_ERR_WORKSPACE;
+    return launch_clip_grad_norm(n, src, src_dtype, dst, dst_dtype, size, max_norm, grad_scale, static_cast<double *>(workspace), norm,
+                                 static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

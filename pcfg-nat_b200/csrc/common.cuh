@@ -162,6 +162,23 @@ int launch_logsoftmax_gather(void *logits, int dtype, const int64_t *sel, int64_
 int launch_logsoftmax_gather_grad(void *probs, int dtype, const float *grad, const int64_t *sel, int64_t sb, int64_t sl,
                                   int64_t ss, int64_t rows, int64_t rpb, int V, int slen, int *status, cudaStream_t st);
 
+int launch_token_logprobs(const void *logits, int dtype, int64_t n, int64_t inner, int64_t stride_outer, int64_t stride_inner, int V,
+                          const int64_t *tokens, int has_ignore, int64_t ignore, int top, float *logprob, float *entropy,
+                          float *top_logprob, int64_t *top_index, float *kept, int *status, cudaStream_t st);
+int launch_token_logprobs_grad(const void *logits, int dtype, int64_t n, int64_t inner, int64_t stride_outer, int64_t stride_inner,
+                               int V, const int64_t *tokens, int has_ignore, int64_t ignore, int top, const float *kept,
+                               const float *entropy, const int64_t *top_index, const float *g_logprob, const float *g_entropy,
+                               const float *g_top, void *dlogits, int64_t pitch, int *status, cudaStream_t st);
+int launch_embed(const void *weight, int dtype, int64_t w_stride, int64_t V, int H, const int64_t *tokens, int64_t n, float scale,
+                 void *out, int *status, cudaStream_t st);
+size_t embed_workspace_bytes(int64_t n, int H);
+int launch_embed_backward(const void *grad, int dtype, int64_t g_stride, const int64_t *tokens, int64_t n, int64_t V, int H, float scale,
+                          int has_padding, int64_t padding, void *dw, int dw_dtype, int64_t dw_stride, int accumulate, void *workspace,
+                          int *status, cudaStream_t st);
+int clip_grad_norm_sums(int n);  // doubles of scratch memory for n tensors
+int launch_clip_grad_norm(int n, const void *const *src, const int *src_dtype, void *const *dst, const int *dst_dtype,
+                          const int64_t *size, float limit, float scale, double *sums, float *norm, cudaStream_t st);
+
 // row-per-thread family on its own; redo != nullptr: only the sentences the linear-space kernels left marked
 int launch_loss_fwd_rows(const float *match_all, const float *links, const int64_t *ol, const int64_t *tl, int B, int L,
                          int T, float *S, float *C, float *loss, int *status, cudaStream_t st, const float *redo);
