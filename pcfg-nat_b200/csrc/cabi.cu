@@ -715,7 +715,7 @@ int pcfgnat_embed(const void *weight, int dtype, int64_t weight_stride, int64_t 
 
 size_t pcfgnat_embed_backward_workspace_bytes(int64_t n, int64_t V, int H) {
     if (n < 0 || V < 1 || H < 1) return 0;
-    return embed_workspace_bytes(n, H);
+    return embed_workspace_bytes(n, V, H);
 }
 
 int pcfgnat_embed_backward(const void *grad_out, int dtype, int64_t grad_stride, const int64_t *tokens, int64_t n, int64_t V,
@@ -726,8 +726,8 @@ int pcfgnat_embed_backward(const void *grad_out, int dtype, int64_t grad_stride,
     if (n < 0 || V < 1 || H < 1 || grad_stride < 0 || d_stride < H) return PCFGNAT_ERR_INVALID_ARGUMENT;
     if (!d_weight || !workspace || (n && (!grad_out || !tokens))) return PCFGNAT_ERR_INVALID_ARGUMENT;
     if (dtype < 0 || dtype > PCFGNAT_DTYPE_BF16 || (d_dtype != PCFGNAT_DTYPE_F32 && d_dtype != dtype)) return PCFGNAT_ERR_UNSUPPORTED;
-    if (n > INT32_MAX || V > INT32_MAX || H > (1 << 28)) return PCFGNAT_ERR_TOO_LARGE;
-    if (workspace_bytes < embed_workspace_bytes(n, H)) return PCFGNAT_ERR_WORKSPACE;
+    if (n > INT32_MAX || V > INT32_MAX || H > (1 << 20)) return PCFGNAT_ERR_TOO_LARGE;
+    if (workspace_bytes < embed_workspace_bytes(n, V, H)) return PCFGNAT_ERR_WORKSPACE;
     return launch_embed_backward(grad_out, dtype, grad_stride, tokens, n, V, H, scale, has_padding != 0, padding_idx, d_weight, d_dtype,
                                  d_stride, accumulate != 0, workspace, status, static_cast<cudaStream_t>(stream));
 }

@@ -171,7 +171,7 @@ int launch_token_logprobs_grad(const void *logits, int dtype, int64_t n, int64_t
                                const float *g_top, void *dlogits, int64_t pitch, int *status, cudaStream_t st);
 int launch_embed(const void *weight, int dtype, int64_t w_stride, int64_t V, int H, const int64_t *tokens, int64_t n, float scale,
                  void *out, int *status, cudaStream_t st);
-size_t embed_workspace_bytes(int64_t n, int H);
+size_t embed_workspace_bytes(int64_t n, int64_t V, int H);
 int launch_embed_backward(const void *grad, int dtype, int64_t g_stride, const int64_t *tokens, int64_t n, int64_t V, int H, float scale,
                           int has_padding, int64_t padding, void *dw, int dw_dtype, int64_t dw_stride, int accumulate, void *workspace,
                           int *status, cudaStream_t st);

@@ -6,7 +6,7 @@
 //      and reads all tokens: those below its range count where its entries begin, so no block waits for another.
 //   2. embed_sum_kernel   — the sorted list cut into pieces of equal length.  A run of one token inside a piece is written
 //      to the table at once; the part of a run that crosses a piece's border goes to scratch memory.
-//   3. embed_join_kernel  — adds up the parts of every run that crosses borders, in the order of the pieces.
+//   3. embed_join_kernel  — adds up the parts of every run that crosses pieces, in an order that its pieces decide.
 // A placeholder that fills most positions is thus spread over as many blocks as its share of the list.
 #include "row_vectors.cuh"
 
@@ -47,43 +47,61 @@ __global__ void __launch_bounds__(kThreads)
 
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kMaxRange = 512;   // rows of the table that one block may own
+constexpr int kAhead = 8;        // loads of 32 tokens that a warp has in flight
 
 __device__ __forceinline__ void zero_row(char *p, int bytes, int lane) {
     if (!((reinterpret_cast<uintptr_t>(p) | (unsigned)bytes) & 15)) {
         for (int i = lane; i < bytes / 16; i += 32) reinterpret_cast<uint4 *>(p)[i] = make_uint4(0, 0, 0, 0);
+    } else if (!((reinterpret_cast<uintptr_t>(p) | (unsigned)bytes) & 3)) {
+        for (int i = lane; i < bytes / 4; i += 32) reinterpret_cast<uint32_t *>(p)[i] = 0;
     } else {
         for (int i = lane; i < bytes / 2; i += 32) reinterpret_cast<uint16_t *>(p)[i] = 0;
     }
 }
 
-// sorted_token / sorted_at: the tokens that count and their positions, sorted; *total their number.  Rows of dw without a
-// token are set to zero where `zero`.
+struct Sorted {
+    int *token, *at;  // the tokens that count and their positions, by token and then by position
+    int *row_end;     // [V] where the list's entries of a token end
+    int *total;       // entries
+};
+
+// Rows of dw without a token are set to zero where `zero`.
 __global__ void __launch_bounds__(kSortThreads)
-    embed_sort_kernel(const int64_t *__restrict__ tokens, int n, int64_t V, int has_padding, int64_t padding, int range,
-                      int *sorted_token, int *sorted_at, int *total, char *dw, int64_t row_bytes, int64_t dw_stride_bytes,
-                      int zero, int *status) {
+    embed_sort_kernel(const int64_t *__restrict__ tokens, int n, int V, int has_padding, int64_t padding, int range, Sorted sorted,
+                      char *dw, int row_bytes, int64_t dw_stride_bytes, int zero, int *status) {
     extern __shared__ int cell[];  // [warp][row of the range]: tokens of the warp's span, then where the next one goes
     __shared__ int warp_sum[kSortWarps], warp_below[kSortWarps];
     __shared__ int counts[kMaxRange];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int64_t v0 = (int64_t)blockIdx.x * range, v1 = min(v0 + range, V);
-    const int rows = (int)(v1 - v0);
+    const int v0 = blockIdx.x * range, rows = min(range, V - v0);
     for (int i = tid; i < kSortWarps * range; i += kSortThreads) cell[i] = 0;
     __syncthreads();
     const int span = ((n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
-    const int first = min((int64_t)warp * span, (int64_t)n), last = min((int64_t)first + span, (int64_t)n);
+    const int first = (int)min((int64_t)warp * span, (int64_t)n), last = (int)min((int64_t)first + span, (int64_t)n);
     int *mine = cell + warp * range;
+    // the token at i, or -1 where it does not count
+    const auto counted = [&](int64_t t) { return t < 0 || t >= V || (has_padding && t == padding) ? -1 : (int)t; };
     int below = 0;
     bool bad = false;
-    for (int i = first + lane; i < last; i += 32) {
-        const int64_t t = tokens[i];
-        if (t < 0 || t >= V) {
-            bad = true;
-            continue;
+    uint64_t seen = 0;  // groups of 32 of the first 64 that hold tokens of the range; later groups are all looked at again
+    int group = 0;
+    for (int i0 = first; i0 < last; i0 += 32 * kAhead) {
+        int64_t t[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const int i = i0 + k * 32 + lane;
+            t[k] = i < last ? tokens[i] : (int64_t)V;
+            if (i < last && (t[k] < 0 || t[k] >= V)) bad = true;
         }
-        if (has_padding && t == padding) continue;
-        if (t < v0) below++;
-        else if (t < v1) atomicAdd(mine + (t - v0), 1);
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const int v = counted(t[k]);
+            const bool in = v >= v0 && v < v0 + rows;
+            below += v >= 0 && v < v0;
+            if (in) atomicAdd(mine + (v - v0), 1);
+            if (__any_sync(0xffffffffu, in) && group < 64) seen |= 1ull << group;
+            group++;
+        }
     }
     if (bad && blockIdx.x == 0) flag(status, PCFGNAT_STATUS_BAD_INDEX);
     below = __reduce_add_sync(0xffffffffu, below);
@@ -102,111 +120,178 @@ __global__ void __launch_bounds__(kSortThreads)
     if (lane == 31) warp_sum[warp] = scan;
     if (tid < kMaxRange) counts[tid] = mine_total;
     __syncthreads();
-    int start = scan - mine_total;
-    for (int w = 0; w < kSortWarps; w++) start += warp_below[w] + (w < warp ? warp_sum[w] : 0);
     if (tid < rows) {
-        int next = start;
+        int next = scan - mine_total;
+        for (int w = 0; w < kSortWarps; w++) next += warp_below[w] + (w < warp ? warp_sum[w] : 0);
         for (int w = 0; w < kSortWarps; w++) {
             const int c = cell[w * range + tid];
             cell[w * range + tid] = next;
             next += c;
         }
-        if (tid == rows - 1 && v1 == V) *total = next;
+        sorted.row_end[v0 + tid] = next;
+        if (v0 + tid == V - 1) *sorted.total = next;
     }
     __syncthreads();
     if (zero)
         for (int r = warp; r < rows; r += kSortWarps)
-            if (counts[r] == 0) zero_row(dw + (v0 + r) * dw_stride_bytes, (int)row_bytes, lane);
-    for (int i0 = first; i0 < last; i0 += 32) {
+            if (counts[r] == 0) zero_row(dw + (v0 + r) * dw_stride_bytes, row_bytes, lane);
+    group = 0;
+    for (int i0 = first; i0 < last; i0 += 32, group++) {
+        if (group < 64 && !(seen >> group & 1)) continue;
         const int i = i0 + lane;
-        const int64_t t = i < last ? tokens[i] : -1;
-        const bool in = t >= v0 && t < v1 && !(has_padding && t == padding);
-        const uint32_t any = __ballot_sync(0xffffffffu, in);
-        if (any == 0) continue;
-        const int row = in ? (int)(t - v0) : -1;
+        const int v = i < last ? counted(tokens[i]) : -1;
+        const bool in = v >= v0 && v < v0 + rows;
+        const int row = in ? v - v0 : -1;
         const uint32_t same = __match_any_sync(0xffffffffu, row);
         int at = 0;
         if (in) at = mine[row] + __popc(same & ((1u << lane) - 1));
         __syncwarp();
         if (in && lane == __ffs(same) - 1) mine[row] += __popc(same);
         __syncwarp();
-        if (in) sorted_token[at] = (int)t, sorted_at[at] = i;
+        if (in) sorted.token[at] = v, sorted.at[at] = i;
     }
 }
 
 template <typename T, int VEC>
 __device__ __forceinline__ void write_row(T *p, const float (&acc)[VEC], float scale, int accumulate) {
-    using Raw = typename RawVec<VEC * sizeof(T)>::type;
-    float x[VEC];
-    if (accumulate) {
-        unpack_vec<T, VEC>(*reinterpret_cast<const Raw *>(p), x);
+    constexpr int kStep = VEC * sizeof(T) > 16 ? 16 / sizeof(T) : VEC;  // numbers of one store
+    using Raw = typename RawVec<kStep * sizeof(T)>::type;
 #pragma unroll
-        for (int k = 0; k < VEC; k++) x[k] += acc[k] * scale;
-    } else {
+    for (int j = 0; j < VEC; j += kStep) {
+        float x[kStep] = {};
+        if (accumulate) unpack_vec<T, kStep>(*reinterpret_cast<const Raw *>(p + j), x);
 #pragma unroll
-        for (int k = 0; k < VEC; k++) x[k] = acc[k] * scale;
+        for (int k = 0; k < kStep; k++) x[k] += acc[j + k] * scale;
+        *reinterpret_cast<Raw *>(p + j) = pack_vec<T, kStep>(x);
     }
-    *reinterpret_cast<Raw *>(p) = pack_vec<T, VEC>(x);
 }
 
+constexpr int kSumWarps = 8;
+
 struct Pieces {
-    const int *sorted_token, *sorted_at, *total;
+    Sorted sorted;
     float *parts;  // [piece][2][H]: what a piece holds of a run that began before it, and of one that goes on behind it
-    int length;    // entries of a piece
+    int length;    // entries of a warp, kSumWarps warps to a piece
 };
 
-// VEC elements of the gradient per thread; a table of another type than the gradient's is written VEC at a time as well.
+// A block adds up a piece of the list for 32 * VEC columns, a warp an equal share of it, a lane VEC columns.  A warp's runs that
+// cross its borders are joined in shared memory, in the list's order, and so are given on only where they cross the piece's.
 template <typename G, typename W, int VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(32 * kSumWarps)
     embed_sum_kernel(const G *__restrict__ grad, int64_t g_stride, int H, Pieces p, W *dw, int64_t dw_stride, float scale,
                      int accumulate) {
     using Raw = typename RawVec<VEC * sizeof(G)>::type;
-    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * VEC;
-    const int total = *p.total;
-    const int64_t begin64 = (int64_t)blockIdx.x * p.length;
-    if (begin64 >= total || c >= H) return;
-    const int begin = (int)begin64, end = min(begin + p.length, total);
-    const int before = begin > 0 ? p.sorted_token[begin - 1] : -1, after = end < total ? p.sorted_token[end] : -1;
-    float *head = p.parts + (int64_t)blockIdx.x * 2 * H + c, *tail = head + H;
-    float acc[VEC] = {};
-    int token = p.sorted_token[begin];
-    bool began_before = token == before;
-    for (int i = begin; i < end; i++) {
-        const int at = p.sorted_at[i];
-        float x[VEC];
-        unpack_vec<G, VEC>(__ldg(reinterpret_cast<const Raw *>(grad + at * g_stride + c)), x);
+    __shared__ float crossing[kSumWarps][2][32 * VEC];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int c = (blockIdx.y * 32 + lane) * VEC;
+    const bool there = c < H;
+    const int total = *p.sorted.total;
+    const int64_t begin64 = ((int64_t)blockIdx.x * kSumWarps + warp) * p.length;
+    const int *token = p.sorted.token;
+    if ((int64_t)blockIdx.x * kSumWarps * p.length >= total) return;
+    if (begin64 < total) {
+        const int begin = (int)begin64, end = min(begin + p.length, total);
+        const int before = begin > 0 ? token[begin - 1] : -1, after = end < total ? token[end] : -1;
+        float acc[VEC] = {};
+        int run = token[begin];
+        bool began_before = run == before;
+        for (int i0 = begin; i0 < end; i0 += 32) {
+            const int count = min(32, end - i0);
+            const int my_token = lane < count ? token[i0 + lane] : -1, my_at = lane < count ? p.sorted.at[i0 + lane] : 0;
+            const int behind = i0 + count < end ? token[i0 + count] : -1;
+            for (int j0 = 0; j0 < count; j0 += kAhead) {
+                Raw raw[kAhead];
 #pragma unroll
-        for (int k = 0; k < VEC; k++) acc[k] += x[k];
-        const int next = i + 1 < end ? p.sorted_token[i + 1] : -1;
-        if (next == token) continue;
-        if (began_before || (i + 1 == end && token == after)) {
-            float *to = began_before ? head : tail;
+                for (int j = 0; j < kAhead; j++) {
+                    const int at = __shfl_sync(0xffffffffu, my_at, (j0 + j) & 31);
+                    if (there && j0 + j < count) raw[j] = __ldg(reinterpret_cast<const Raw *>(grad + at * g_stride + c));
+                }
 #pragma unroll
-            for (int k = 0; k < VEC; k++) to[k] = acc[k];
-        } else {
-            write_row<W, VEC>(dw + token * dw_stride + c, acc, scale, accumulate);
+                for (int j = 0; j < kAhead; j++) {
+                    const int next_of = __shfl_sync(0xffffffffu, my_token, (j0 + j + 1) & 31);
+                    if (j0 + j < count) {  // the same for the whole warp
+                        float x[VEC];
+                        unpack_vec<G, VEC>(raw[j], x);
+#pragma unroll
+                        for (int k = 0; k < VEC; k++) acc[k] += x[k];
+                        const bool last = j0 + j + 1 == count;
+                        const int next = last ? behind : next_of;
+                        if (next != run) {
+                            const bool goes_on = next < 0 && run == after;
+                            if (began_before || goes_on) {
+                                float *to = crossing[warp][began_before ? 0 : 1] + lane * VEC;
+#pragma unroll
+                                for (int k = 0; k < VEC; k++) to[k] = acc[k];
+                            } else if (there) {
+                                write_row<W, VEC>(dw + run * dw_stride + c, acc, scale, accumulate);
+                            }
+#pragma unroll
+                            for (int k = 0; k < VEC; k++) acc[k] = 0.f;
+                            run = next;
+                            began_before = false;
+                        }
+                    }
+                }
+            }
         }
-#pragma unroll
-        for (int k = 0; k < VEC; k++) acc[k] = 0.f;
-        token = next;
-        began_before = false;
+    }
+    __syncthreads();
+    // 32 * VEC columns by as many threads: what the warps left, in the list's order
+    for (int col = threadIdx.x; col < 32 * VEC; col += 32 * kSumWarps) {
+        const int cc = blockIdx.y * 32 * VEC + col;
+        if (cc >= H) continue;
+        float *give = p.parts + (int64_t)blockIdx.x * 2 * H + cc;
+        float acc[1] = {0.f};
+        bool from_outside = false, open = false;
+        for (int w = 0; w < kSumWarps; w++) {
+            const int64_t b64 = ((int64_t)blockIdx.x * kSumWarps + w) * p.length;
+            if (b64 >= total) break;
+            const int b = (int)b64, e = min(b + p.length, total);
+            const int head = token[b], tail = token[e - 1];
+            const bool before = b > 0 && token[b - 1] == head, behind = e < total && token[e] == tail;
+            if (before) {
+                if (w == 0) from_outside = true;
+                acc[0] += crossing[w][0][col];
+                open = head == tail && behind;
+                if (!open) {
+                    if (from_outside) give[0] = acc[0];
+                    else write_row<W, 1>(dw + head * dw_stride + cc, acc, scale, accumulate);
+                    acc[0] = 0.f;
+                    from_outside = false;
+                }
+            }
+            if (behind && !(before && head == tail)) acc[0] = crossing[w][1][col], open = true;
+        }
+        if (open) give[from_outside ? 0 : H] = acc[0];
     }
 }
 
+// The runs that cross pieces: the first part, and those of the pieces behind it in eight sums of every eighth one.
 template <typename W>
-__global__ void __launch_bounds__(kThreads)
-    embed_join_kernel(int H, Pieces p, W *dw, int64_t dw_stride, float scale, int accumulate) {
-    const int total = *p.total;
-    const int64_t begin64 = (int64_t)blockIdx.x * p.length;
-    const int c = blockIdx.y * kThreads + threadIdx.x;
-    if (begin64 + p.length >= total || c >= H) return;
-    const int begin = (int)begin64, end = begin + p.length;
-    const int token = p.sorted_token[end - 1];
-    if (p.sorted_token[end] != token || (begin > 0 && p.sorted_token[begin - 1] == token)) return;
-    float acc[1] = {p.parts[(int64_t)blockIdx.x * 2 * H + H + c]};
-    for (int64_t q = blockIdx.x + 1; q * p.length < total && p.sorted_token[q * p.length] == token; q++)
-        acc[0] += p.parts[q * 2 * H + c];
-    write_row<W, 1>(dw + token * dw_stride + c, acc, scale, accumulate);
+__global__ void __launch_bounds__(kThreads) embed_join_kernel(int H, Pieces p, W *dw, int64_t dw_stride, float scale, int accumulate) {
+    __shared__ float sums[8][33];
+    const int total = *p.sorted.total, length = p.length * kSumWarps;
+    const int64_t begin64 = (int64_t)blockIdx.x * length;
+    if (begin64 + length >= total) return;
+    const int begin = (int)begin64, end = begin + length;
+    const int token = p.sorted.token[end - 1];
+    if (p.sorted.token[end] != token || (begin > 0 && p.sorted.token[begin - 1] == token)) return;
+    const int last = (p.sorted.row_end[token] - 1) / length;  // the piece in which the run ends
+    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, c = blockIdx.y * 32 + lane;
+    float acc = 0.f;
+    if (c < H) {
+        if (group == 0) acc = p.parts[(int64_t)blockIdx.x * 2 * H + H + c];
+#pragma unroll 8
+        for (int64_t q = (int64_t)blockIdx.x + 1 + group; q <= last; q += 8) acc += p.parts[q * 2 * H + c];
+    }
+    sums[group][lane] = acc;
+    __syncthreads();
+    if (group == 0 && c < H) {
+        float sum[1] = {0.f};
+#pragma unroll
+        for (int g = 0; g < 8; g++) sum[0] += sums[g][lane];
+        write_row<W, 1>(dw + token * dw_stride + c, sum, scale, accumulate);
+    }
 }
 
 int widest(uintptr_t bits, int size) {  // bytes of the widest vector that addresses and strides allow, at least an element's
@@ -215,18 +300,22 @@ int widest(uintptr_t bits, int size) {  // bytes of the widest vector that addre
     return size;
 }
 
-int piece_length(int64_t n) {
-    const int64_t even = (n + 2047) / 2048;  // at most 2 048 pieces
-    return (int)(even < 16 ? 16 : even);
+// Entries of a warp: eight loads of a lane in flight, more where that made over 2 048 pieces.
+int warp_entries(int64_t n) {
+    const int64_t even = (n + 2048 * kSumWarps - 1) / (2048 * kSumWarps);
+    return (int)((even + kAhead - 1) / kAhead * kAhead) + (even == 0 ? kAhead : 0);
 }
-int64_t piece_count(int64_t n) { return (n + piece_length(n) - 1) / piece_length(n); }
+int64_t piece_count(int64_t n) {
+    const int64_t length = (int64_t)warp_entries(n) * kSumWarps;
+    return (n + length - 1) / length;
+}
 
 constexpr size_t round16(size_t x) { return (x + 15) / 16 * 16; }
 
 }  // namespace
 
-size_t embed_workspace_bytes(int64_t n, int H) {
-    return 16 + 2 * round16((size_t)n * sizeof(int)) + (size_t)piece_count(n) * 2 * H * sizeof(float);
+size_t embed_workspace_bytes(int64_t n, int64_t V, int H) {
+    return 16 + 2 * round16((size_t)n * sizeof(int)) + round16((size_t)V * sizeof(int)) + (size_t)piece_count(n) * 2 * H * sizeof(float);
 }
 
 int launch_embed(const void *weight, int dtype, int64_t w_stride, int64_t V, int H, const int64_t *tokens, int64_t n, float scale,
@@ -257,10 +346,10 @@ int launch_embed_backward(const void *grad, int dtype, int64_t g_stride, const i
                           int has_padding, int64_t padding, void *dw, int dw_dtype, int64_t dw_stride, int accumulate, void *workspace,
                           int *status, cudaStream_t st) {
     char *ws = static_cast<char *>(workspace);
-    int *total = reinterpret_cast<int *>(ws);
-    int *sorted_token = reinterpret_cast<int *>(ws + 16);
-    int *sorted_at = reinterpret_cast<int *>(ws + 16 + round16((size_t)n * sizeof(int)));
-    float *parts = reinterpret_cast<float *>(ws + 16 + 2 * round16((size_t)n * sizeof(int)));
+    const size_t list = round16((size_t)n * sizeof(int));
+    const Sorted sorted{reinterpret_cast<int *>(ws + 16), reinterpret_cast<int *>(ws + 16 + list),
+                        reinterpret_cast<int *>(ws + 16 + 2 * list), reinterpret_cast<int *>(ws)};
+    float *parts = reinterpret_cast<float *>(ws + 16 + 2 * list + round16((size_t)V * sizeof(int)));
     const size_t dw_size = dw_dtype == PCFGNAT_DTYPE_F32 ? 4 : 2;
     const int64_t per_sm = (V + sm_count() - 1) / sm_count();
     const int range = (int)(per_sm < kMaxRange ? per_sm : kMaxRange);
@@ -268,35 +357,33 @@ int launch_embed_backward(const void *grad, int dtype, int64_t g_stride, const i
     cudaError_t e = ensure_dynamic_smem(embed_sort_kernel, smem);
     if (e != cudaSuccess) return PCFGNAT_ERR_CUDA;
     embed_sort_kernel<<<(unsigned)((V + range - 1) / range), kSortThreads, smem, st>>>(
-        tokens, (int)n, V, has_padding, padding, range, sorted_token, sorted_at, total, static_cast<char *>(dw), (int64_t)(H * dw_size),
+        tokens, (int)n, (int)V, has_padding, padding, range, sorted, static_cast<char *>(dw), (int)(H * dw_size),
         (int64_t)(dw_stride * dw_size), !accumulate, status);
     e = cudaGetLastError();
     if (e != cudaSuccess || n == 0) return cuda_rc(e);
-    const Pieces p{sorted_token, sorted_at, total, parts, piece_length(n)};
+    const Pieces p{sorted, parts, warp_entries(n)};
     const unsigned pieces = (unsigned)piece_count(n);
     return with_dtype(dtype, [&](auto g) {
         using G = decltype(g);
         const auto run = [&](auto w) {
             using W = decltype(w);
-            // one vector width for both: the gradient's rows in 16 bytes, the table's in as many elements
+            // a lane's columns: as many of the gradient's as 16 bytes hold, where both rows' addresses allow whole vectors
             const auto bits = [&](const void *a, int64_t stride, size_t size) {
                 return reinterpret_cast<uintptr_t>(a) | (uintptr_t)(stride * size) | (uintptr_t)(H * size);
             };
             const int wide_g = widest(bits(grad, g_stride, sizeof(G)), sizeof(G)) / (int)sizeof(G);
             const int wide_w = widest(bits(dw, dw_stride, sizeof(W)), sizeof(W)) / (int)sizeof(W);
-            const int wide = wide_g < wide_w ? wide_g : wide_w;
             const auto sum = [&](auto vec) {
                 constexpr int VEC = decltype(vec)::value;
-                const int chunks = H / VEC;
-                const int threads = chunks >= kThreads ? kThreads : (chunks + 31) / 32 * 32;
-                embed_sum_kernel<G, W, VEC><<<dim3(pieces, (unsigned)((chunks + threads - 1) / threads)), threads, 0, st>>>(
+                embed_sum_kernel<G, W, VEC><<<dim3(pieces, (unsigned)((H / VEC + 31) / 32)), 32 * kSumWarps, 0, st>>>(
                     static_cast<const G *>(grad), g_stride, H, p, static_cast<W *>(dw), dw_stride, scale, accumulate);
             };
-            if (wide >= 4) sum(std::integral_constant<int, 4>());
-            else if (wide >= 2) sum(std::integral_constant<int, 2>());
+            constexpr int kWide = 16 / sizeof(G), kWideW = 16 / sizeof(W) < kWide ? 16 / sizeof(W) : kWide;
+            if (wide_g >= kWide && wide_w >= kWideW && H % kWide == 0) sum(std::integral_constant<int, kWide>());
+            else if (wide_g >= 2 && wide_w >= 2) sum(std::integral_constant<int, 2>());
             else sum(std::integral_constant<int, 1>());
-            embed_join_kernel<W><<<dim3(pieces, (unsigned)((H + kThreads - 1) / kThreads)), kThreads, 0, st>>>(
-                H, p, static_cast<W *>(dw), dw_stride, scale, accumulate);
+            embed_join_kernel<W><<<dim3(pieces, (unsigned)((H + 31) / 32)), kThreads, 0, st>>>(H, p, static_cast<W *>(dw), dw_stride,
+                                                                                             scale, accumulate);
             return cuda_rc(cudaGetLastError());
         };
         if (dw_dtype == PCFGNAT_DTYPE_F32) return run(float());

@@ -3,6 +3,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace pcfgnat {
@@ -76,6 +78,63 @@ __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two floats for the packed instructions, each result rounded as by itself.
+struct Packed {
+    unsigned long long bits;
+    __device__ __forceinline__ Packed(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(x), "f"(y)); }
+    __device__ __forceinline__ Packed operator+(const Packed &o) const {
+        Packed r = *this;
+        asm("add.rn.f32x2 %0, %0, %1;" : "+l"(r.bits) : "l"(o.bits));
+        return r;
+    }
+    __device__ __forceinline__ Packed operator*(const Packed &o) const {
+        Packed r = *this;
+        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(r.bits) : "l"(o.bits));
+        return r;
+    }
+    __device__ __forceinline__ float2 get() const {
+        float2 v;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(bits));
+        return v;
+    }
+};
+__device__ __forceinline__ Packed fma(const Packed &a, const Packed &b, const Packed &c) {
+    Packed r = a;
+    asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(r.bits) : "l"(b.bits), "l"(c.bits));
+    return r;
+}
+
+// The pair of numbers that begins at 32-bit word k: two halves of one word, or two words.
+template <typename T>
+__device__ __forceinline__ Packed pair_of_words(const uint32_t *word, int k) {
+    if constexpr (sizeof(T) == 4) {
+        return Packed(__uint_as_float(word[k]), __uint_as_float(word[k + 1]));
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        return Packed(__uint_as_float(word[k] << 16), __uint_as_float(word[k] & 0xffff0000u));
+    } else {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(word + k));
+        return Packed(v.x, v.y);
+    }
+}
+// The largest number in N words; NaN if there is one.
+template <typename T, int N>
+__device__ __forceinline__ float max_of_words(const uint32_t *word) {
+    uint32_t m = word[0];
+#pragma unroll
+    for (int k = 1; k < N; k++) {
+        if constexpr (sizeof(T) == 4) asm("max.NaN.f32 %0, %0, %1;" : "+r"(m) : "r"(word[k]));
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(word[k]));
+        else asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(m) : "r"(word[k]));
+    }
+    if constexpr (sizeof(T) == 4) return __uint_as_float(m);
+    const float2 v = pair_of_words<T>(&m, 0).get();
+    return max_nan(v.x, v.y);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t neg_inf_word() {
+    return sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __nv_bfloat16> ? 0xff80ff80u : 0xfc00fc00u;
 }
 
 // Calls f with a value of the C++ type of a PCFGNAT_DTYPE_*.

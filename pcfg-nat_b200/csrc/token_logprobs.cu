@@ -9,18 +9,21 @@
 //
 // The `top` largest values (equal ones by rising index) need no second pass: the top-th largest of the threads' maxima is a
 // lower bound of the top-th largest value, so only the few threads whose maximum reaches it look at their numbers again.
+#include <cooperative_groups.h>
+
+#include <algorithm>
 #include <cfloat>
 
 #include "row_vectors.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace pcfgnat {
 
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kUnroll = 4;            // 16-byte loads of a thread in flight
 constexpr int kMaxTop = PCFGNAT_MAX_TOP;
-constexpr int kCandidates = 512;      // values that reach the bound; more are handled one at a time
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFarBelow = -1.0e4f;  // 2^x of anything smaller is 0, and 0 * x stays 0 (with -inf it would be NaN)
 
@@ -43,18 +46,41 @@ __device__ __forceinline__ Stats join(Stats a, Stats b) {
     a.u += b.u;
     return a;
 }
-template <int N>
-__device__ __forceinline__ void take(Stats &a, const float (&x)[N]) {
-    float m = a.m;
+
+// One number of a row.
+template <bool ENTROPY>
+__device__ __forceinline__ void take_one(Stats &a, float x) {
+    rescale(a, max_nan(a.m, x));
+    const float d = max_nan((x - a.m) * kLog2e, kFarBelow), e = exp2_approx(d);
+    a.s += e;
+    if (ENTROPY) a.u += e * d;
+}
+
+// kUnroll vectors of a row: one maximum and one rescaling for all, then two numbers at a time.
+template <typename T, bool ENTROPY>
+__device__ __forceinline__ void take(Stats &a, const uint4 (&raw)[kUnroll]) {
+    constexpr int kWords = 4 * kUnroll;
+    uint32_t word[kWords];
 #pragma unroll
-    for (int k = 0; k < N; k++) m = max_nan(m, x[k]);
-    rescale(a, m);
-#pragma unroll
-    for (int k = 0; k < N; k++) {
-        const float d = max_nan((x[k] - m) * kLog2e, kFarBelow), e = exp2_approx(d);
-        a.s += e;
-        a.u += e * d;
+    for (int k = 0; k < kUnroll; k++) {
+        word[4 * k] = raw[k].x, word[4 * k + 1] = raw[k].y, word[4 * k + 2] = raw[k].z, word[4 * k + 3] = raw[k].w;
     }
+    rescale(a, max_nan(a.m, max_of_words<T, kWords>(word)));
+    const Packed minus_m(-a.m, -a.m), log2e(kLog2e, kLog2e);
+    Packed s(0.f, 0.f), u(0.f, 0.f);
+    constexpr int kStep = sizeof(T) == 4 ? 2 : 1;
+#pragma unroll
+    for (int k = 0; k < kWords; k += kStep) {
+        const Packed y = (pair_of_words<T>(word, k) + minus_m) * log2e;
+        float2 d = y.get();
+        if (ENTROPY) d.x = max_nan(d.x, kFarBelow), d.y = max_nan(d.y, kFarBelow);
+        const Packed e(exp2_approx(d.x), exp2_approx(d.y));
+        s = s + e;
+        if (ENTROPY) u = fma(e, Packed(d.x, d.y), u);
+    }
+    const float2 s2 = s.get(), u2 = u.get();
+    a.s += s2.x + s2.y;
+    if (ENTROPY) a.u += u2.x + u2.y;
 }
 
 // Order-preserving integers of floats (no NaN among them).
@@ -62,7 +88,7 @@ __device__ __forceinline__ uint32_t rank_bits(float x) {
     const uint32_t b = __float_as_uint(x + 0.f);  // -0 equals +0
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-// One key per entry: larger value first, then smaller index.
+// One key per entry: larger value first, then smaller index.  No entry has key 0.
 __device__ __forceinline__ uint64_t entry_key(float x, int index) {
     return (uint64_t)rank_bits(x) << 32 | (uint32_t)~index;
 }
@@ -82,98 +108,59 @@ struct Rows {
     }
 };
 
+struct Given {
+    const int64_t *tokens;
+    int64_t ignore;
+    int has_ignore;
+};
+
+struct Results {
+    int top;
+    float *logprob, *entropy, *top_logprob;
+    int64_t *top_index;
+    float *kept;
+    int *status;
+};
+
+// The numbers of a row that one team of threads looks at.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    token_logprobs_kernel(Rows rows, const int64_t *__restrict__ tokens, int has_ignore, int64_t ignore, int top,
-                          float *logprob, float *entropy, float *top_logprob, int64_t *top_index, float *kept, int *status) {
-    constexpr int kVec = RowCut<T>::kVec;
-    __shared__ Stats part[kWarps];
-    __shared__ uint32_t maxima[kThreads];
-    __shared__ uint64_t found[kCandidates];
-    __shared__ int n_found;
-    __shared__ uint32_t bound;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int64_t r = blockIdx.x;
-    const int V = rows.V;
-    const int64_t token = tokens[r];
-    if (has_ignore && token == ignore) {
-        if (tid == 0) {
-            logprob[r] = 0.f;
-            if (entropy) entropy[r] = 0.f;
-            if (kept) kept[2 * r] = kept[2 * r + 1] = 0.f;
-        }
-        if (tid < top) top_logprob[r * top + tid] = 0.f, top_index[r * top + tid] = -1;
-        return;
-    }
-    const T *row = rows.at<T>(r);
-    const RowCut<T> cut(row, V);
-    const uint4 *vec = reinterpret_cast<const uint4 *>(row + cut.head);
-    Stats a;
-    {
-        int i = tid;
-        for (; i + (kUnroll - 1) * kThreads < cut.vecs; i += kUnroll * kThreads) {
-            uint4 raw[kUnroll];
-#pragma unroll
-            for (int k = 0; k < kUnroll; k++) raw[k] = __ldg(vec + i + k * kThreads);
-#pragma unroll
-            for (int k = 0; k < kUnroll; k++) {
-                float x[kVec];
-                unpack_vec<T, kVec>(raw[k], x);
-                take(a, x);
-            }
-        }
-        for (; i < cut.vecs; i += kThreads) {
-            float x[kVec];
-            unpack_vec<T, kVec>(__ldg(vec + i), x);
-            take(a, x);
-        }
-        if (tid < cut.loose(V)) {
-            float x[1] = {num_to_float<T>(row[cut.loose_at(tid)])};
-            take(a, x);
-        }
-    }
-    const float own_max = a.m;
-    const bool own_any = a.s > 0.f;  // some entry that is not -inf
-    if (tid == 0) n_found = 0;
-    maxima[tid] = own_any ? rank_bits(own_max) : 0u;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Stats b;
-        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-        b.u = __shfl_xor_sync(0xffffffffu, a.u, o);
-        a = join(a, b);
-    }
-    if (lane == 0) part[warp] = a;
-    __syncthreads();
-    a = part[0];
-#pragma unroll
-    for (int w = 1; w < kWarps; w++) a = join(a, part[w]);
-    const float log_s = logf(a.s);  // -inf for a row of nothing but -inf
-    if (tid == 0) {
-        float lp;
-        if (token < 0 || token >= V) {
-            lp = CUDART_NAN_F;
-            flag(status, PCFGNAT_STATUS_BAD_INDEX);
-        } else {
-            const float x = num_to_float<T>(row[token]);
-            lp = a.s == 0.f ? neg_inf() : (x - a.m) - log_s;
-        }
-        logprob[r] = lp;
-        if (entropy) entropy[r] = a.s == 0.f ? 0.f : log_s - kLn2 * (a.u / a.s);
-        if (kept) kept[2 * r] = a.m, kept[2 * r + 1] = log_s;
-    }
-    if (top == 0) return;
-    if (!(a.s > 0.f)) {  // no distribution, or nothing in it
-        if (tid < top) top_logprob[r * top + tid] = a.s == 0.f ? neg_inf() : a.s, top_index[r * top + tid] = -1;
-        return;
-    }
+struct Part {
+    const T *row;
+    const uint4 *vec;
+    int head, first, last;  // vectors [first, last)
+    int loose, vecs;        // numbers in no vector that this part takes, vectors of the whole row
+    __device__ __forceinline__ int loose_at(int i) const { return i < head ? i : i + vecs * RowCut<T>::kVec; }
+};
+
+// What a team of NT threads shares.
+template <int NT>
+struct Team {
+    static constexpr int kWarps = NT / 32;
+    static constexpr int kCandidates = NT == 32 ? 128 : 512;  // values that reach the bound; more are found one at a time
+    Stats part[kWarps];
+    uint32_t maxima[NT];
+    uint64_t found[kCandidates];
+    uint64_t best[kMaxTop];
+    Stats whole;
+    int n_found;
+    uint32_t bound;
+};
+
+template <int NT>
+__device__ __forceinline__ void team_sync() {
+    if (NT == 32) __syncwarp();
+    else __syncthreads();
+}
+
+// The `top` best entries of a part, sorted, into t.best (0 where there are fewer).
+template <typename T, int NT>
+__device__ void best_entries(Team<NT> &t, const Part<T> &p, int top, uint32_t own_max, int tid) {
+    constexpr int kVec = RowCut<T>::kVec, kWarps = Team<NT>::kWarps;
+    const int warp = tid >> 5, lane = tid & 31;
     if (warp == 0) {  // the top-th largest of the threads' maxima
-        uint32_t v[kWarps];
-        uint32_t best = 0;
+        uint32_t v[kWarps], best = 0, at = 0;
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) v[w] = maxima[w * 32 + lane], best = max(best, v[w]);
-        uint32_t at = 0;
+        for (int w = 0; w < kWarps; w++) v[w] = t.maxima[w * 32 + lane], best = max(best, v[w]);
         for (int k = 0; k < top; k++) {
             at = __reduce_max_sync(0xffffffffu, best);
             if (at == 0) break;  // fewer threads than that saw anything: every number is a candidate
@@ -188,76 +175,195 @@ __global__ void __launch_bounds__(kThreads)
                 }
             }
         }
-        if (lane == 0) bound = at;
+        if (lane == 0) t.bound = at;
+        if (lane < top) t.best[lane] = 0;
     }
-    __syncthreads();
-    const uint32_t least = bound;
-    const uint32_t again = __ballot_sync(0xffffffffu, own_any && rank_bits(own_max) >= least);
+    team_sync<NT>();
+    const uint32_t least = t.bound;
     const auto offer = [&](float x, int index) {
         if (x == neg_inf() || rank_bits(x) < least) return;
-        const int at = atomicAdd(&n_found, 1);
-        if (at < kCandidates) found[at] = entry_key(x, index);
+        const int at = atomicAdd(&t.n_found, 1);
+        if (at < Team<NT>::kCandidates) t.found[at] = entry_key(x, index);
     };
-    for (uint32_t todo = again; todo; todo &= todo - 1) {
-        const int of = warp * 32 + __ffs(todo) - 1;
-        for (int i = of + lane * kThreads; i < cut.vecs; i += 32 * kThreads) {
+    for (uint32_t todo = __ballot_sync(0xffffffffu, own_max != 0 && own_max >= least); todo; todo &= todo - 1) {
+        const int of = warp * 32 + __ffs(todo) - 1;  // the whole warp looks at this thread's numbers
+        for (int i = p.first + of + lane * NT; i < p.last; i += 32 * NT) {
             float x[kVec];
-            unpack_vec<T, kVec>(__ldg(vec + i), x);
+            unpack_vec<T, kVec>(__ldg(p.vec + i), x);
 #pragma unroll
-            for (int k = 0; k < kVec; k++) offer(x[k], cut.head + i * kVec + k);
+            for (int k = 0; k < kVec; k++) offer(x[k], p.head + i * kVec + k);
         }
-        if (lane == 0 && of < cut.loose(V)) {
-            const int i = cut.loose_at(of);
-            offer(num_to_float<T>(row[i]), i);
+        if (lane == 0 && of < p.loose) {
+            const int i = p.loose_at(of);
+            offer(num_to_float<T>(p.row[i]), i);
         }
     }
-    __syncthreads();
-    const int n = n_found;
-    if (n <= kCandidates) {
-        for (int i = tid; i < n; i += kThreads) {
-            const uint64_t key = found[i];
+    team_sync<NT>();
+    const int n = t.n_found;
+    if (n <= Team<NT>::kCandidates) {
+        for (int i = tid; i < n; i += NT) {
+            const uint64_t key = t.found[i];
             int better = 0;
-            for (int j = 0; j < n; j++) better += found[j] > key;
-            if (better < top) {
-                top_logprob[r * top + better] = (key_value(key) - a.m) - log_s;
-                top_index[r * top + better] = key_index(key);
-            }
+            for (int j = 0; j < n; j++) better += t.found[j] > key;
+            if (better < top) t.best[better] = key;
         }
-        if (tid >= n && tid < top) top_logprob[r * top + tid] = neg_inf(), top_index[r * top + tid] = -1;
         return;
     }
-    // Many equal values at the bound: one sweep over the row per alternative.
+    // Many equal values at the bound, or few threads that saw any: one sweep over the part per alternative.
     uint64_t last = ~0ull;
     for (int k = 0; k < top; k++) {
         uint64_t best = 0;
-        for (int i = tid; i < V; i += kThreads) {
-            const float x = num_to_float<T>(row[i]);
-            const uint64_t key = entry_key(x, i);
+        const auto look = [&](float x, int index) {
+            const uint64_t key = entry_key(x, index);
             if (x != neg_inf() && key < last && key > best) best = key;
+        };
+        for (int i = p.first + tid; i < p.last; i += NT) {
+            float x[kVec];
+            unpack_vec<T, kVec>(__ldg(p.vec + i), x);
+#pragma unroll
+            for (int j = 0; j < kVec; j++) look(x[j], p.head + i * kVec + j);
         }
+        if (tid < p.loose) look(num_to_float<T>(p.row[p.loose_at(tid)]), p.loose_at(tid));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
             best = other > best ? other : best;
         }
-        __syncthreads();
-        if (lane == 0) found[warp] = best;
-        __syncthreads();
-        for (int w = 0; w < kWarps; w++) best = found[w] > best ? found[w] : best;
-        if (tid == 0) {
-            top_logprob[r * top + k] = (key_value(best) - a.m) - log_s;
-            top_index[r * top + k] = key_index(best);
-        }
+        team_sync<NT>();
+        if (lane == 0) t.found[warp] = best;
+        team_sync<NT>();
+        for (int w = 0; w < kWarps; w++) best = t.found[w] > best ? t.found[w] : best;
+        if (tid == 0) t.best[k] = best;
         last = best;
     }
 }
 
+// A team of NT threads per row or, in a cluster, per part of a row; the first block of a cluster joins the parts.
+template <typename T, int NT, bool ENTROPY>
+__global__ void __launch_bounds__(NT < 128 ? 128 : NT)
+    token_logprobs_kernel(Rows rows, int64_t n_rows, Given given, Results out) {
+    constexpr int kTeams = NT < 128 ? 128 / NT : 1;
+    __shared__ Team<NT> teams[kTeams];
+    Team<NT> &t = teams[kTeams == 1 ? 0 : threadIdx.x / NT];
+    const int tid = threadIdx.x % NT, warp = tid >> 5, lane = tid & 31;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int parts = kTeams == 1 ? (int)cluster.num_blocks() : 1, rank = kTeams == 1 ? (int)cluster.block_rank() : 0;
+    const int64_t r = kTeams == 1 ? (int64_t)(blockIdx.x / (unsigned)parts) : (int64_t)blockIdx.x * kTeams + threadIdx.x / NT;
+    if (r >= n_rows) return;
+    const int V = rows.V, top = out.top;
+    const int64_t token = given.tokens[r];
+    if (given.has_ignore && token == given.ignore) {
+        if (rank) return;
+        if (tid == 0) {
+            out.logprob[r] = 0.f;
+            if (out.entropy) out.entropy[r] = 0.f;
+            if (out.kept) out.kept[2 * r] = out.kept[2 * r + 1] = 0.f;
+        }
+        if (tid < top) out.top_logprob[r * top + tid] = 0.f, out.top_index[r * top + tid] = -1;
+        return;
+    }
+    Part<T> p;
+    {
+        p.row = rows.at<T>(r);
+        const RowCut<T> cut(p.row, V);
+        p.head = cut.head, p.vecs = cut.vecs;
+        p.vec = reinterpret_cast<const uint4 *>(p.row + cut.head);
+        const int share = (cut.vecs + parts - 1) / parts;
+        p.first = min(rank * share, cut.vecs), p.last = min(p.first + share, cut.vecs);
+        p.loose = rank == 0 ? cut.loose(V) : 0;
+    }
+    Stats a;
+    for (int i = p.first + tid; i < p.last; i += kUnroll * NT) {
+        uint4 raw[kUnroll];
+#pragma unroll
+        for (int k = 0; k < kUnroll; k++) {
+            const uint32_t none = neg_inf_word<T>();
+            raw[k] = i + k * NT < p.last ? __ldg(p.vec + i + k * NT) : make_uint4(none, none, none, none);
+        }
+        take<T, ENTROPY>(a, raw);
+    }
+    if (tid < p.loose) take_one<ENTROPY>(a, num_to_float<T>(p.row[p.loose_at(tid)]));
+    const uint32_t own_max = a.s > 0.f ? rank_bits(a.m) : 0u;  // 0: no entry but -inf (or NaN, where nothing is chosen)
+    t.maxima[tid] = own_max;
+    if (tid == 0) t.n_found = 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        Stats b;
+        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
+        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
+        b.u = __shfl_xor_sync(0xffffffffu, a.u, o);
+        a = join(a, b);
+    }
+    if (Team<NT>::kWarps > 1) {
+        if (lane == 0) t.part[warp] = a;
+        team_sync<NT>();
+        a = t.part[0];
+#pragma unroll
+        for (int w = 1; w < Team<NT>::kWarps; w++) a = join(a, t.part[w]);
+    } else {
+        team_sync<NT>();
+    }
+    if (top) {
+        if (a.s > 0.f) best_entries<T, NT>(t, p, top, own_max, tid);
+        else if (tid < top) t.best[tid] = 0;
+    }
+    int n_best = top;
+    if (parts > 1) {
+        if (tid == 0) t.whole = a;
+        cluster.sync();
+        if (rank == 0) {
+            for (int q = 1; q < parts; q++) a = join(a, *cluster.map_shared_rank(&t.whole, q));
+            if (top) {  // the parts' best entries side by side
+                n_best = parts * top;
+                for (int i = tid; i < n_best; i += NT) t.found[i] = cluster.map_shared_rank(t.best, i / top)[i % top];
+                __syncthreads();
+                if (tid < top) t.best[tid] = 0;
+                __syncthreads();
+            }
+        }
+        cluster.sync();  // a block's memory is there until it has been read
+        if (rank) return;
+        if (top) {
+            for (int i = tid; i < n_best; i += NT) {
+                const uint64_t key = t.found[i];
+                int better = 0;
+                for (int j = 0; j < n_best; j++) better += t.found[j] > key;
+                if (key && better < top) t.best[better] = key;
+            }
+            __syncthreads();
+        }
+    } else if (top) {
+        team_sync<NT>();
+    }
+    const float log_s = logf(a.s);  // -inf for a row of nothing but -inf
+    if (tid == 0) {
+        float lp;
+        if (token < 0 || token >= V) {
+            lp = CUDART_NAN_F;
+            flag(out.status, PCFGNAT_STATUS_BAD_INDEX);
+        } else {
+            lp = a.s == 0.f ? neg_inf() : (num_to_float<T>(p.row[token]) - a.m) - log_s;
+        }
+        out.logprob[r] = lp;
+        if (ENTROPY) out.entropy[r] = a.s == 0.f ? 0.f : log_s - kLn2 * (a.u / a.s);
+        if (out.kept) out.kept[2 * r] = a.m, out.kept[2 * r + 1] = log_s;
+    }
+    if (tid < top) {
+        const uint64_t key = a.s > 0.f ? t.best[tid] : 0;
+        // a row that is no distribution is NaN; an alternative that does not exist has no probability
+        out.top_logprob[r * top + tid] = key ? (key_value(key) - a.m) - log_s : a.s >= 0.f ? neg_inf() : CUDART_NAN_F;
+        out.top_index[r * top + tid] = key ? key_index(key) : -1;
+    }
+}
+
+constexpr int kThreads = 256;
+
 // d x_v = p_v (-G - h (log p_v + H)) + sum of the gradients given to v, G their sum over the row, h the entropy's.
 // The few entries that tokens and alternatives name are formed again, with what is added, before they are rounded.
+// A block per row, or per part of a row (blockIdx.y) where the rows alone do not fill the GPU.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    token_logprobs_grad_kernel(Rows rows, const int64_t *__restrict__ tokens, int has_ignore, int64_t ignore, int top,
-                               const float *__restrict__ kept, const float *__restrict__ entropy,
+    token_logprobs_grad_kernel(Rows rows, Given given, int top, const float *__restrict__ kept, const float *__restrict__ entropy,
                                const int64_t *__restrict__ top_index, const float *__restrict__ g_logprob,
                                const float *__restrict__ g_entropy, const float *__restrict__ g_top, T *dlogits, int64_t pitch,
                                int *status) {
@@ -269,8 +375,8 @@ __global__ void __launch_bounds__(kThreads)
     const int V = rows.V;
     const T *row = rows.at<T>(r);
     T *out = dlogits + r * pitch;
-    const int64_t token = tokens[r];
-    const bool left_out = has_ignore && token == ignore;
+    const int64_t token = given.tokens[r];
+    const bool left_out = given.has_ignore && token == given.ignore;
     const float m = kept[2 * r], log_s = kept[2 * r + 1];
     const bool bad = !left_out && g_logprob && (token < 0 || token >= V);
     if (bad && tid == 0) flag(status, PCFGNAT_STATUS_BAD_INDEX);
@@ -279,7 +385,7 @@ __global__ void __launch_bounds__(kThreads)
         float g = 0.f;
         if (tid == 0 && g_logprob) index = token, g = g_logprob[r];
         if (tid > 0 && tid <= top && g_top) index = top_index[r * top + tid - 1], g = index < 0 ? 0.f : g_top[r * top + tid - 1];
-        at[tid] = (int)index;
+        at[tid] = index < 0 || index >= V ? -1 : (int)index;
         add[tid] = g;
     }
     __syncthreads();
@@ -293,33 +399,58 @@ __global__ void __launch_bounds__(kThreads)
         const float lp = max_nan((x - m) - log_s, kFarBelow);
         return exp2_approx(lp * kLog2e) * (base - h * lp);
     };
+    const Packed minus_m(-m, -m), minus_log_s(-log_s, -log_s), log2e(kLog2e, kLog2e), base2(base, base), minus_h(-h, -h);
+    const auto grad_vec = [&](const uint4 &raw) {
+        uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int k = 0; k < 4; k += sizeof(T) == 4 ? 2 : 1) {
+            float2 lp = (pair_of_words<T>(word, k) + minus_m + minus_log_s).get();
+            lp.x = max_nan(lp.x, kFarBelow), lp.y = max_nan(lp.y, kFarBelow);
+            const Packed lp2(lp.x, lp.y);
+            const float2 y = (lp2 * log2e).get();
+            const float2 d = (Packed(exp2_approx(y.x), exp2_approx(y.y)) * fma(minus_h, lp2, base2)).get();
+            if constexpr (sizeof(T) == 4) word[k] = __float_as_uint(d.x), word[k + 1] = __float_as_uint(d.y);
+            else word[k] = pack_vec<T, 2>({d.x, d.y});
+        }
+        return make_uint4(word[0], word[1], word[2], word[3]);
+    };
     const RowCut<T> cut(out, V);
     const bool same = !((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15);
-    if (zero || same) {
-        const uint4 *vec = reinterpret_cast<const uint4 *>(row + cut.head);
-        uint4 *to = reinterpret_cast<uint4 *>(out + cut.head);
-        for (int i = tid; i < cut.vecs; i += kThreads) {
-            float x[kVec] = {};
-            if (!zero) {
-                unpack_vec<T, kVec>(__ldg(vec + i), x);
-#pragma unroll
-                for (int k = 0; k < kVec; k++) x[k] = grad(x[k]);
-            }
-            to[i] = pack_vec<T, kVec>(x);
-        }
-        if (tid < cut.loose(V)) {
-            const int i = cut.loose_at(tid);
-            out[i] = num_from_float<T>(zero ? 0.f : grad(num_to_float<T>(row[i])));
-        }
-    } else {
-        for (int i = tid; i < V; i += kThreads) out[i] = num_from_float<T>(grad(num_to_float<T>(row[i])));
+    // this block's part: vectors [first, last), with the numbers in no vector in the first one
+    const int share = (cut.vecs + gridDim.y - 1) / gridDim.y;
+    const int first = min((int)blockIdx.y * share, cut.vecs), last = min(first + share, cut.vecs);
+    if (tid < (blockIdx.y == 0 ? cut.loose(V) : 0)) {
+        const int i = cut.loose_at(tid);
+        out[i] = num_from_float<T>(zero ? 0.f : grad(num_to_float<T>(row[i])));
     }
-    if (zero) return;
+    uint4 *to = reinterpret_cast<uint4 *>(out + cut.head);
+    if (zero) {
+        for (int i = first + tid; i < last; i += kThreads) to[i] = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    if (same) {
+        const uint4 *vec = reinterpret_cast<const uint4 *>(row + cut.head);
+        int i = first + tid;
+        for (; i + (kUnroll - 1) * kThreads < last; i += kUnroll * kThreads) {
+            uint4 raw[kUnroll];
+#pragma unroll
+            for (int k = 0; k < kUnroll; k++) raw[k] = __ldg(vec + i + k * kThreads);
+#pragma unroll
+            for (int k = 0; k < kUnroll; k++) to[i + k * kThreads] = grad_vec(raw[k]);
+        }
+        for (; i < last; i += kThreads) to[i] = grad_vec(__ldg(vec + i));
+    } else {  // rows that begin at different places of a 16-byte vector
+        for (int i = first * kVec + tid; i < last * kVec; i += kThreads)
+            out[cut.head + i] = num_from_float<T>(grad(num_to_float<T>(row[cut.head + i])));
+    }
     __syncthreads();
-    if (tid <= top && at[tid] >= 0 && at[tid] < V) {
-        float g = 0.f;
-        for (int k = 0; k <= top; k++) g += at[k] == at[tid] ? add[k] : 0.f;
-        out[at[tid]] = num_from_float<T>(grad(num_to_float<T>(row[at[tid]])) + g);
+    if (tid <= top && at[tid] >= 0) {
+        const int i = at[tid], v = i < cut.head || i >= cut.head + cut.vecs * kVec ? -1 : (i - cut.head) / kVec;
+        if (v < 0 ? blockIdx.y == 0 : v >= first && v < last) {  // written by this block
+            float g = 0.f;
+            for (int k = 0; k <= top; k++) g += at[k] == i ? add[k] : 0.f;
+            out[i] = num_from_float<T>(grad(num_to_float<T>(row[i])) + g);
+        }
     }
 }
 
@@ -330,11 +461,34 @@ int launch_token_logprobs(const void *logits, int dtype, int64_t n, int64_t inne
                           float *top_logprob, int64_t *top_index, float *kept, int *status, cudaStream_t st) {
     if (n == 0) return PCFGNAT_OK;
     const Rows rows{logits, inner, stride_outer, stride_inner, V};
+    const Given given{tokens, ignore, has_ignore};
+    const Results out{top, logprob, entropy, top_logprob, top_index, kept, status};
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        token_logprobs_kernel<T><<<(unsigned)n, kThreads, 0, st>>>(rows, tokens, has_ignore, ignore, top, logprob, entropy,
-                                                                   top_logprob, top_index, kept, status);
-        return cuda_rc(cudaGetLastError());
+        const int64_t vecs = V / RowCut<T>::kVec, sms = sm_count();
+        const auto run = [&](auto team, int parts) {
+            constexpr int NT = decltype(team)::value;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)(NT < 128 ? (n * NT + 127) / 128 : n * parts));
+            cfg.blockDim = dim3(NT < 128 ? 128 : NT);
+            cfg.stream = st;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = (unsigned)parts;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = parts > 1 ? 1 : 0;
+            return cuda_rc(entropy ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT, true>, rows, n, given, out)
+                                   : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT, false>, rows, n, given, out));
+        };
+        // A warp per row while a lane has no more than eight vectors; else a block of 128 threads, and up to eight blocks per row
+        // where the rows alone do not fill the GPU and every thread of them still has two vectors.
+        if (vecs <= 256) return run(std::integral_constant<int, 32>(), 1);
+        int parts = 1;
+        while (parts < 8 && n * parts * 2 <= 8 * sms && vecs >= (int64_t)parts * 2 * 256) parts *= 2;
+        if (n * parts > INT32_MAX) return (int)PCFGNAT_ERR_TOO_LARGE;
+        if (parts == 8 && n * parts <= sms && vecs >= 8 * 1024) return run(std::integral_constant<int, 512>(), parts);
+        return run(std::integral_constant<int, 128>(), parts);
     });
 }
 
@@ -344,11 +498,14 @@ int launch_token_logprobs_grad(const void *logits, int dtype, int64_t n, int64_t
                                const float *g_top, void *dlogits, int64_t pitch, int *status, cudaStream_t st) {
     if (n == 0) return PCFGNAT_OK;
     const Rows rows{logits, inner, stride_outer, stride_inner, V};
+    const Given given{tokens, ignore, has_ignore};
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        token_logprobs_grad_kernel<T><<<(unsigned)n, kThreads, 0, st>>>(rows, tokens, has_ignore, ignore, top, kept, entropy, top_index,
-                                                                        g_logprob, g_entropy, g_top, static_cast<T *>(dlogits), pitch,
-                                                                        status);
+        // parts of at least two vectors per thread while there are fewer blocks than the GPU holds at once
+        const int64_t vecs = V / RowCut<T>::kVec, room = 8 * (int64_t)sm_count() / n;
+        const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({room, vecs / (2 * kThreads), 64}));
+        token_logprobs_grad_kernel<T><<<dim3((unsigned)n, (unsigned)parts), kThreads, 0, st>>>(
+            rows, given, top, kept, entropy, top_index, g_logprob, g_entropy, g_top, static_cast<T *>(dlogits), pitch, status);
         return cuda_rc(cudaGetLastError());
     });
 }

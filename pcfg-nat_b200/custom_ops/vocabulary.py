@@ -12,7 +12,7 @@ step of ``runtime.GlanceStep``; its gradient can be added onto the projection's 
 The arguments are checked, outputs allocated with torch, and the kernels run on the tensors' device and its current stream;
 nothing is copied to the host.  There is no CPU path.
 """
-import ctypes
+import array
 import math
 from collections import namedtuple
 
@@ -33,13 +33,30 @@ def _numbers(t, name):
     """The PCFGNAT_DTYPE_* of a CUDA tensor of floating numbers."""
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name} must be a tensor")
-    _ops._require_cuda()
     if not t.is_cuda:
+        _ops._require_cuda()
         raise RuntimeError(f"{name} must be a CUDA tensor")
     dt = _DTYPES.get(t.dtype)
     if dt is None:
         raise RuntimeError(f"{name} must be float32, float16 or bfloat16 (got {t.dtype})")
     return dt
+
+
+class _Stay:
+    """What ``_on`` gives for the current device: switching to it costs more than a small kernel."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *_):
+        pass
+
+
+_STAY = _Stay()
+
+
+def _on(dev):
+    return _STAY if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _token_tensor(tokens, dev, shape=None):
@@ -112,7 +129,7 @@ def _token_logprobs(logits, tokens, top, entropy, ignore, keep):
     shape = logits.shape[:-1]
     tokens = _token_tensor(tokens, dev, shape)
     n = tokens.numel()
-    with torch.cuda.device(dev):
+    with _on(dev):
         new = lambda *more, dtype=torch.float32: torch.empty(shape + more, dtype=dtype, device=dev)
         logprob = new()
         ent = new() if entropy else None
@@ -154,7 +171,7 @@ class TokenLogprobsFunc(Function):
         cont = lambda g: None if g is None else g.contiguous()
         g_logprob, g_entropy, g_top = cont(g_logprob), cont(g_entropy), cont(g_top)
         ptr = lambda t: t.data_ptr() if t is not None else None
-        with torch.cuda.device(dev):
+        with _on(dev):
             d = torch.empty(logits.shape[:-1] + (pitch,), dtype=logits.dtype, device=dev)
             rc = _cabi.lib().pcfgnat_token_logprobs_backward(
                 logits.data_ptr(), _DTYPES[logits.dtype], n, inner, stride_outer, stride_inner, V, tokens.data_ptr(), *ctx.ignore,
@@ -206,7 +223,7 @@ def _embed(weight, tokens, scale):
     dt, dev = _table(weight, "weight"), weight.device
     tokens = _token_tensor(tokens, dev)
     V, H = weight.shape
-    with torch.cuda.device(dev):
+    with _on(dev):
         out = torch.empty(tokens.shape + (H,), dtype=weight.dtype, device=dev)
         rc = _cabi.lib().pcfgnat_embed(weight.data_ptr(), dt, weight.stride(0), V, H, tokens.data_ptr(), tokens.numel(), scale,
                                        out.data_ptr(), _status_of(dev), _ops._stream(dev))
@@ -225,7 +242,7 @@ def _embed_backward(grad_out, tokens, d_weight, scale, padding, accumulate):
         rows = (n, 0, H)
     lib = _cabi.lib()
     nbytes = lib.pcfgnat_embed_backward_workspace_bytes(n, V, H)
-    with torch.cuda.device(dev):
+    with _on(dev):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         rc = lib.pcfgnat_embed_backward(g.data_ptr(), dt, rows[2], tokens.data_ptr(), n, V, H, scale, *padding, d_weight.data_ptr(),
                                         _DTYPES[d_weight.dtype], max(d_weight.stride(0), H), int(accumulate), ws.data_ptr(), nbytes,
@@ -247,7 +264,7 @@ class EmbedTokensFunc(Function):
         if not ctx.needs_input_grad[0]:
             return None, None, None, None
         (tokens,) = ctx.saved_tensors
-        with torch.cuda.device(grad_out.device):
+        with _on(grad_out.device):
             d = torch.empty(ctx.table, dtype=grad_out.dtype, device=grad_out.device)
         return _embed_backward(grad_out, tokens.contiguous(), d, ctx.scale, ctx.padding, False), None, None, None
 
@@ -301,7 +318,7 @@ def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
     """Clips gradients by their global norm, as the trainer does between the backward pass and the optimizer.
 
     norm = ``grad_scale`` * sqrt(sum of all squares); every gradient is multiplied by grad_scale * min(1, max_norm / (norm +
-    1e-6)), in place, or into the tensors ``out`` of the same shapes (each of its gradient's type or float32: half-precision
+    1e-6)), in place, or into the tensors ``out`` of as many numbers each (of its gradient's type or float32: half-precision
     gradients into float32 master gradients, with ``grad_scale`` = 1 / loss scale).  ``grads``: a tensor or an iterable of
     tensors of one device, float32, float16 or bfloat16 mixed, any number of them, in any dense layout; None among them is skipped
     (with its output).  Returns the norm before clipping, a float32 tensor on the device; nothing is read back.
@@ -319,36 +336,46 @@ def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
     if len(outs) != len(grads):
         raise RuntimeError("out must hold one tensor per gradient")
     if any(g is None for g in grads):
-        outs = [o for g, o in zip(grads, outs) if g is not None]
-        grads = [g for g in grads if g is not None]
+        there = [i for i, g in enumerate(grads) if g is not None]
+        grads, outs = [grads[i] for i in there], [outs[i] for i in there]
+        outs = grads if out is None else outs
     if not grads:
         return torch.zeros((), dtype=torch.float32, device=torch.device("cuda", torch.cuda.current_device()))
-    src = [_numbers(g, "a gradient") for g in grads]
-    dev = grads[0].device
-    for g in grads:
-        if g.device != dev:
-            raise RuntimeError("the gradients must be on one device")
-        if not g.is_contiguous() and not _dense(g):
-            raise RuntimeError("a gradient must be dense: call contiguous() first")
-    dst = src
-    if outs is not grads:
-        dst = [_numbers(o, "an output") for o in outs]
+    # one plain pass over the list for each question: a model has hundreds of gradients, and the kernels are done with them sooner
+    every = grads if outs is grads else grads + outs
+    try:
+        at, size = list(map(torch.Tensor.data_ptr, every)), list(map(torch.Tensor.numel, every))
+        index = set(map(torch.Tensor.get_device, every))
+    except TypeError:
+        raise RuntimeError("gradients and outputs must be tensors") from None
+    n = len(grads)
+    if len(index) != 1 or min(index) < 0:
+        raise RuntimeError("the gradients and outputs must be CUDA tensors on one device")
+    kind = [_DTYPES.get(t.dtype) for t in every]
+    if None in kind:
+        raise RuntimeError("gradients and outputs must be float32, float16 or bfloat16")
+    if not all(map(torch.Tensor.is_contiguous, every)):
         for g, o in zip(grads, outs):
-            if o.device != dev or o.shape != g.shape or o.dtype not in (torch.float32, g.dtype):
-                raise RuntimeError("an output must have its gradient's device and shape, and its type or float32")
+            if not _dense(g):
+                raise RuntimeError("a gradient must be dense: call contiguous() first")
             if o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
                 raise RuntimeError("an output must have its gradient's layout")
-    n = len(grads)
+    if outs is not grads:
+        if size[:n] != size[n:]:
+            raise RuntimeError("an output must have its gradient's shape")
+        if any(k and k != j for j, k in zip(kind[:n], kind[n:])):
+            raise RuntimeError("an output must be of its gradient's type or float32")
+    dev = grads[0].device
     lib = _cabi.lib()
-    pointers, ints, longs = ctypes.c_void_p * n, ctypes.c_int * n, ctypes.c_int64 * n
-    at = [g.data_ptr() for g in grads]
-    with torch.cuda.device(dev):
+    host = lambda code, v: array.array(code, v)  # read before the call returns
+    src, dst, src_kind, dst_kind, numel = host("Q", at[:n]), host("Q", at[-n:]), host("i", kind[:n]), host("i", kind[-n:]), host("q", size[:n])
+    head = lambda a: a.buffer_info()[0]
+    with _on(dev):
         nbytes = lib.pcfgnat_clip_grad_norm_workspace_bytes(n)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
-        rc = lib.pcfgnat_clip_grad_norm(n, pointers(*at), ints(*src), pointers(*(at if outs is grads else [o.data_ptr() for o in outs])),
-                                        ints(*dst), longs(*[g.numel() for g in grads]), max_norm, grad_scale, ws.data_ptr(), nbytes,
-                                        norm.data_ptr(), _ops._stream(dev))
+        rc = lib.pcfgnat_clip_grad_norm(n, head(src), head(src_kind), head(dst), head(dst_kind), head(numel), max_norm, grad_scale,
+                                        ws.data_ptr(), nbytes, norm.data_ptr(), _ops._stream(dev))
     if rc == _cabi.ERR_INVALID_ARGUMENT:
         raise RuntimeError("the outputs must not overlap one another or another gradient")
     _cabi.check(rc, "pcfgnat_clip_grad_norm")
