@@ -18,28 +18,28 @@ constexpr int kThreads = 256;
 
 // ---- forward
 
+// A row by a group of `lanes` lanes (a power of two, at most a warp).
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kThreads)
     embed_rows_kernel(const T *__restrict__ weight, int64_t w_stride, int64_t V, int H, const int64_t *__restrict__ tokens,
-                      int64_t n, float scale, T *__restrict__ out, int *status) {
+                      int64_t n, int lanes, float scale, T *__restrict__ out, int *status) {
     using Raw = typename RawVec<VEC * sizeof(T)>::type;
-    const int per_row = H / VEC;
-    const int64_t total = n * per_row;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-        const int64_t r = i / per_row;
-        const int c = (int)(i - r * per_row);
-        const int64_t t = tokens[r];
+    const int lane = threadIdx.x & (lanes - 1);
+    const int64_t r = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / lanes;
+    if (r >= n) return;
+    const int64_t t = tokens[r];
+    const bool bad = t < 0 || t >= V;
+    if (bad && lane == 0) flag(status, PCFGNAT_STATUS_BAD_INDEX);
+    const float factor = bad ? CUDART_NAN_F : scale;
+    const Raw *from = reinterpret_cast<const Raw *>(weight + (bad ? 0 : t) * w_stride);
+    Raw *to = reinterpret_cast<Raw *>(out + r * H);
+#pragma unroll 4
+    for (int c = lane; c < H / VEC; c += lanes) {
         float x[VEC];
-        if (t < 0 || t >= V) {
+        unpack_vec<T, VEC>(__ldg(from + c), x);
 #pragma unroll
-            for (int k = 0; k < VEC; k++) x[k] = CUDART_NAN_F;
-            if (c == 0) flag(status, PCFGNAT_STATUS_BAD_INDEX);
-        } else {
-            unpack_vec<T, VEC>(__ldg(reinterpret_cast<const Raw *>(weight + t * w_stride) + c), x);
-#pragma unroll
-            for (int k = 0; k < VEC; k++) x[k] *= scale;
-        }
-        reinterpret_cast<Raw *>(out + r * H)[c] = pack_vec<T, VEC>(x);
+        for (int k = 0; k < VEC; k++) x[k] *= factor;
+        to[c] = pack_vec<T, VEC>(x);
     }
 }
 
@@ -136,19 +136,28 @@ __global__ void __launch_bounds__(kSortThreads)
         for (int r = warp; r < rows; r += kSortWarps)
             if (counts[r] == 0) zero_row(dw + (v0 + r) * dw_stride_bytes, row_bytes, lane);
     group = 0;
-    for (int i0 = first; i0 < last; i0 += 32, group++) {
-        if (group < 64 && !(seen >> group & 1)) continue;
-        const int i = i0 + lane;
-        const int v = i < last ? counted(tokens[i]) : -1;
-        const bool in = v >= v0 && v < v0 + rows;
-        const int row = in ? v - v0 : -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, row);
-        int at = 0;
-        if (in) at = mine[row] + __popc(same & ((1u << lane) - 1));
-        __syncwarp();
-        if (in && lane == __ffs(same) - 1) mine[row] += __popc(same);
-        __syncwarp();
-        if (in) sorted.token[at] = v, sorted.at[at] = i;
+    for (int i0 = first; i0 < last; i0 += 32 * kAhead, group += kAhead) {
+        const uint32_t some = group < 64 ? (uint32_t)(seen >> group) & ((1u << kAhead) - 1) : (1u << kAhead) - 1;
+        if (!some) continue;
+        int v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const int i = i0 + k * 32 + lane;
+            v[k] = (some >> k & 1) && i < last ? counted(tokens[i]) : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            if (!(some >> k & 1)) continue;
+            const bool in = v[k] >= v0 && v[k] < v0 + rows;
+            const int row = in ? v[k] - v0 : -1;
+            const uint32_t same = __match_any_sync(0xffffffffu, row);
+            int at = 0;
+            if (in) at = mine[row] + __popc(same & ((1u << lane) - 1));
+            __syncwarp();
+            if (in && lane == __ffs(same) - 1) mine[row] += __popc(same);
+            __syncwarp();
+            if (in) sorted.token[at] = v[k], sorted.at[at] = i0 + k * 32 + lane;
+        }
     }
 }
 
@@ -327,10 +336,12 @@ int launch_embed(const void *weight, int dtype, int64_t w_stride, int64_t V, int
                                (uintptr_t)(w_stride * sizeof(T)) | (uintptr_t)(H * sizeof(T));
         const auto run = [&](auto vec) {
             constexpr int VEC = decltype(vec)::value;
-            const int64_t blocks = (n * (H / VEC) + kThreads - 1) / kThreads;
-            const int64_t most = (int64_t)sm_count() * 32;
-            embed_rows_kernel<T, VEC><<<(unsigned)(blocks < most ? blocks : most), kThreads, 0, st>>>(
-                static_cast<const T *>(weight), w_stride, V, H, tokens, n, scale, static_cast<T *>(out), status);
+            int lanes = 1;
+            while (lanes < 32 && lanes < H / VEC) lanes *= 2;
+            const int64_t blocks = (n * lanes + kThreads - 1) / kThreads;
+            if (blocks > INT32_MAX) return (int)PCFGNAT_ERR_TOO_LARGE;
+            embed_rows_kernel<T, VEC><<<(unsigned)blocks, kThreads, 0, st>>>(static_cast<const T *>(weight), w_stride, V, H, tokens, n,
+                                                                             lanes, scale, static_cast<T *>(out), status);
             return cuda_rc(cudaGetLastError());
         };
         switch (widest(bits, sizeof(T))) {
@@ -382,7 +393,8 @@ int launch_embed_backward(const void *grad, int dtype, int64_t g_stride, const i
             if (wide_g >= kWide && wide_w >= kWideW && H % kWide == 0) sum(std::integral_constant<int, kWide>());
             else if (wide_g >= 2 && wide_w >= 2) sum(std::integral_constant<int, 2>());
             else sum(std::integral_constant<int, 1>());
-            embed_join_kernel<W><<<dim3(pieces, (unsigned)((H + 31) / 32)), kThreads, 0, st>>>(H, p, static_cast<W *>(dw), dw_stride,
+            if (pieces > 1)  // one piece has no border
+                embed_join_kernel<W><<<dim3(pieces, (unsigned)((H + 31) / 32)), kThreads, 0, st>>>(H, p, static_cast<W *>(dw), dw_stride,
                                                                                              scale, accumulate);
             return cuda_rc(cudaGetLastError());
         };

@@ -16,25 +16,35 @@ constexpr int kBlocksPerSm = 4;
 constexpr int kChunk = 8192;        // numbers that a block takes at a time
 constexpr int kMaxTensors = 1024;   // of one launch: 29 bytes each of the 32 764 that parameters may have
 
+// N is a few sizes, so that a short list does not pay for the parameters of a long one.
+template <int N>
 struct Tensors {
-    const void *src[kMaxTensors];
-    void *dst[kMaxTensors];
-    int64_t size[kMaxTensors];
-    int first_chunk[kMaxTensors];  // chunks of the tensors before it
-    uint8_t kind[kMaxTensors];     // type of src, and of dst times 4
-    int count, chunks;
+    const void *src[N];
+    void *dst[N];
+    int64_t size[N];
+    int first_chunk[N];  // chunks of the tensors before it
+    uint8_t kind[N];     // type of src, and of dst times 4
+    int count, chunks, all_in_place;
 };
 
-// The tensor that a chunk belongs to.
-__device__ __forceinline__ int tensor_of(const Tensors &t, int chunk) {
-    int lo = 0, hi = t.count - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (t.first_chunk[mid] <= chunk) lo = mid;
-        else hi = mid - 1;
+// Which tensor a chunk belongs to, by a search in shared memory.
+template <int N>
+struct ChunkMap {
+    int first_chunk[N];
+    __device__ __forceinline__ void fill(const Tensors<N> &t) {
+        for (int i = threadIdx.x; i < t.count; i += kThreads) first_chunk[i] = t.first_chunk[i];
+        __syncthreads();
     }
-    return lo;
-}
+    __device__ __forceinline__ int tensor_of(int chunk, int count) const {
+        int lo = 0, hi = count - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2;
+            if (first_chunk[mid] <= chunk) lo = mid;
+            else hi = mid - 1;
+        }
+        return lo;
+    }
+};
 
 template <class F>
 __device__ __forceinline__ void with_type(int kind, F f) {
@@ -53,12 +63,37 @@ __device__ __forceinline__ double block_sum(double v, double *part) {
     return v;
 }
 
-__global__ void __launch_bounds__(kThreads) grad_squares_kernel(const __grid_constant__ Tensors t, double *sums) {
+// The squares of a vector's numbers.  Those of half-precision numbers have at most 22 bits: in float32 every product is exact and
+// a sum of eight is rounded seven times; the sum is added in 64 bits.  bfloat16 numbers have the range of float32, so sums that
+// left float32's range, or come near its lower end, are formed again in 64 bits.
+template <typename T>
+__device__ __forceinline__ double squares(const uint4 &raw) {
+    constexpr int kVec = RowCut<T>::kVec;
+    float x[kVec];
+    unpack_vec<T, kVec>(raw, x);
+    if constexpr (sizeof(T) == 2) {
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < kVec; j++) s = fmaf(x[j], x[j], s);
+        if (std::is_same_v<T, __half> || (s >= 1e-25f && s <= 1e37f)) return s;
+        if (((raw.x | raw.y | raw.z | raw.w) & 0x7fff7fffu) == 0) return 0.0;
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < kVec; j++) sum += (double)x[j] * (double)x[j];
+    return sum;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kThreads) grad_squares_kernel(const __grid_constant__ Tensors<N> t, double *sums) {
     __shared__ double part[kThreads / 32];
+    __shared__ ChunkMap<N> map;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the next kernel waits for this one's end all the same
+    map.fill(t);
     const int tid = threadIdx.x;
     double sum = 0.0;
     for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const int k = tensor_of(t, c);
+        const int k = map.tensor_of(c, t.count);
         const int64_t begin = (int64_t)(c - t.first_chunk[k]) * kChunk;
         const int n = (int)min((int64_t)kChunk, t.size[k] - begin);
         with_type(t.kind[k] & 3, [&](auto type) {
@@ -67,13 +102,15 @@ __global__ void __launch_bounds__(kThreads) grad_squares_kernel(const __grid_con
             const T *src = static_cast<const T *>(t.src[k]) + begin;
             const RowCut<T> cut(src, n);
             const uint4 *vec = reinterpret_cast<const uint4 *>(src + cut.head);
-#pragma unroll 4
-            for (int i = tid; i < cut.vecs; i += kThreads) {
-                float x[kVec];
-                unpack_vec<T, kVec>(__ldg(vec + i), x);
+            int i = tid;
+            for (; i + 3 * kThreads < cut.vecs; i += 4 * kThreads) {
+                uint4 raw[4];
 #pragma unroll
-                for (int j = 0; j < kVec; j++) sum += (double)x[j] * (double)x[j];
+                for (int j = 0; j < 4; j++) raw[j] = __ldg(vec + i + j * kThreads);
+#pragma unroll
+                for (int j = 0; j < 4; j++) sum += squares<T>(raw[j]);
             }
+            for (; i < cut.vecs; i += kThreads) sum += squares<T>(__ldg(vec + i));
             if (tid < cut.loose(n)) {
                 const double x = num_to_float<T>(src[cut.loose_at(tid)]);
                 sum += x * x;
@@ -84,11 +121,14 @@ __global__ void __launch_bounds__(kThreads) grad_squares_kernel(const __grid_con
     if (tid == 0) sums[blockIdx.x] = sum;
 }
 
+template <int N>
 __global__ void __launch_bounds__(kThreads)
-    grad_scale_kernel(const __grid_constant__ Tensors t, const double *__restrict__ sums, int n_sums, float limit, float scale,
-                      float *norm_out) {
+    grad_scale_kernel(const __grid_constant__ Tensors<N> t, const double *sums, int n_sums, float limit, float scale, float *norm_out) {
     __shared__ double part[kThreads / 32];
+    __shared__ ChunkMap<N> map;
+    map.fill(t);
     const int tid = threadIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched while the sums are still formed
     double sum = 0.0;
     for (int i = tid; i < n_sums; i += kThreads) sum += sums[i];
     sum = block_sum(sum, part);
@@ -96,8 +136,9 @@ __global__ void __launch_bounds__(kThreads)
     if (norm_out && blockIdx.x == 0 && tid == 0) *norm_out = norm;
     const float part_of = limit / (norm + 1e-6f);
     const float factor = (part_of >= 1.f ? 1.f : part_of) * scale;  // NaN stays NaN
+    if (factor == 1.f && t.all_in_place) return;
     for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {  // what was read last is still in L2
-        const int k = tensor_of(t, c);
+        const int k = map.tensor_of(c, t.count);
         if (factor == 1.f && t.src[k] == t.dst[k]) continue;
         const int64_t begin = (int64_t)(c - t.first_chunk[k]) * kChunk;
         const int n = (int)min((int64_t)kChunk, t.size[k] - begin);
@@ -122,7 +163,8 @@ __global__ void __launch_bounds__(kThreads)
                             float y[kOut];
 #pragma unroll
                             for (int q = 0; q < kOut; q++) y[q] = x[j + q];
-                            reinterpret_cast<uint4 *>(dst + cut.head + i * kVec + j)[0] = pack_vec<D, kOut>(y);
+                            // not read again here: it should not push out what is still to be read
+                            __stcs(reinterpret_cast<uint4 *>(dst + cut.head + i * kVec + j), pack_vec<D, kOut>(y));
                         }
                     }
                     if (tid < cut.loose(n)) {
@@ -145,37 +187,68 @@ int clip_grad_norm_sums(int n) {  // doubles of scratch memory for n tensors
     return kBlocksPerSm * sm_count() * ((n + kMaxTensors - 1) / kMaxTensors);
 }
 
-int launch_clip_grad_norm(int n, const void *const *src, const int *src_dtype, void *const *dst, const int *dst_dtype,
-                          const int64_t *size, float limit, float scale, double *sums, float *norm, cudaStream_t st) {
+namespace {
+
+// Both launches' parameters for the tensors [first, first + count); false where a chunk's number does not fit.
+template <int N>
+bool describe(Tensors<N> &t, int first, int count, const void *const *src, const int *src_dtype, void *const *dst, const int *dst_dtype,
+              const int64_t *size) {
+    int64_t chunks = 0;
+    t.count = count, t.all_in_place = 1;
+    for (int i = 0; i < count; i++) {
+        t.src[i] = src[first + i], t.dst[i] = dst[first + i], t.size[i] = size[first + i];
+        t.kind[i] = (uint8_t)(src_dtype[first + i] | dst_dtype[first + i] << 2);
+        t.first_chunk[i] = (int)chunks;
+        if (t.src[i] != t.dst[i]) t.all_in_place = 0;
+        chunks += (t.size[i] + kChunk - 1) / kChunk;
+        if (chunks > 0x3fffffff) return false;
+    }
+    t.chunks = (int)chunks;
+    return true;
+}
+
+template <int N>
+int clip_all(int n, const void *const *src, const int *src_dtype, void *const *dst, const int *dst_dtype, const int64_t *size,
+             float limit, float scale, double *sums, float *norm, cudaStream_t st) {
     const int blocks = kBlocksPerSm * sm_count();
     int n_sums = 0;
-    Tensors t;
-    for (int pass = 0; pass < 2; pass++) {
-        bool norm_written = false;
-        for (int first = 0; first < n || (pass == 1 && !norm_written); first += kMaxTensors) {
-            int64_t chunks = 0;
-            t.count = 0;
-            for (int i = first; i < n && i < first + kMaxTensors; i++) {
-                t.src[t.count] = src[i], t.dst[t.count] = dst[i], t.size[t.count] = size[i];
-                t.kind[t.count] = (uint8_t)(src_dtype[i] | dst_dtype[i] << 2);
-                t.first_chunk[t.count++] = (int)chunks;
-                chunks += (size[i] + kChunk - 1) / kChunk;
-                if (chunks > 0x3fffffff) return PCFGNAT_ERR_TOO_LARGE;
-            }
-            t.chunks = (int)chunks;
-            const int grid = chunks < blocks ? (chunks > 0 ? (int)chunks : 1) : blocks;
-            if (pass == 0) {
-                grad_squares_kernel<<<grid, kThreads, 0, st>>>(t, sums + n_sums);
-                n_sums += grid;
-            } else {
-                grad_scale_kernel<<<grid, kThreads, 0, st>>>(t, sums, n_sums, limit, scale, norm_written ? nullptr : norm);
-                norm_written = true;
-            }
-            const cudaError_t e = cudaGetLastError();
-            if (e != cudaSuccess) return PCFGNAT_ERR_CUDA;
-        }
+    Tensors<N> t;
+    const auto next = [&](int first) {  // describes the tensors from `first` on; blocks of their launches, -1: too many chunks
+        if (!describe(t, first, n - first < N ? n - first : N, src, src_dtype, dst, dst_dtype, size)) return -1;
+        return t.chunks < 1 ? 1 : t.chunks < blocks ? t.chunks : blocks;
+    };
+    for (int first = 0; first < n; first += N) {
+        const int grid = next(first);
+        if (grid < 0) return PCFGNAT_ERR_TOO_LARGE;
+        grad_squares_kernel<N><<<grid, kThreads, 0, st>>>(t, sums + n_sums);
+        n_sums += grid;
+        if (cudaGetLastError() != cudaSuccess) return PCFGNAT_ERR_CUDA;
+    }
+    for (int first = 0; first < n || first == 0; first += N) {
+        const int grid = n > N || n == 0 ? next(first) : n_sums;  // what a single launch was told is still there
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)grid);
+        cfg.blockDim = dim3(kThreads);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, grad_scale_kernel<N>, t, (const double *)sums, n_sums, limit, scale,
+                                                 first == 0 ? norm : (float *)nullptr);
+        if (e != cudaSuccess) return PCFGNAT_ERR_CUDA;
     }
     return PCFGNAT_OK;
+}
+
+}  // namespace
+
+int launch_clip_grad_norm(int n, const void *const *src, const int *src_dtype, void *const *dst, const int *dst_dtype,
+                          const int64_t *size, float limit, float scale, double *sums, float *norm, cudaStream_t st) {
+    if (n <= 64) return clip_all<64>(n, src, src_dtype, dst, dst_dtype, size, limit, scale, sums, norm, st);
+    if (n <= 320) return clip_all<320>(n, src, src_dtype, dst, dst_dtype, size, limit, scale, sums, norm, st);
+    return clip_all<kMaxTensors>(n, src, src_dtype, dst, dst_dtype, size, limit, scale, sums, norm, st);
 }
 
 }  // namespace pcfgnat

@@ -139,10 +139,11 @@ struct Team {
     static constexpr int kCandidates = NT == 32 ? 128 : 512;  // values that reach the bound; more are found one at a time
     Stats part[kWarps];
     uint32_t maxima[NT];
+    uint16_t again[NT];  // threads whose numbers are looked at once more
     uint64_t found[kCandidates];
     uint64_t best[kMaxTop];
     Stats whole;
-    int n_found;
+    int n_found, n_again;
     uint32_t bound;
 };
 
@@ -185,19 +186,29 @@ __device__ void best_entries(Team<NT> &t, const Part<T> &p, int top, uint32_t ow
         const int at = atomicAdd(&t.n_found, 1);
         if (at < Team<NT>::kCandidates) t.found[at] = entry_key(x, index);
     };
-    for (uint32_t todo = __ballot_sync(0xffffffffu, own_max != 0 && own_max >= least); todo; todo &= todo - 1) {
-        const int of = warp * 32 + __ffs(todo) - 1;  // the whole warp looks at this thread's numbers
-        for (int i = p.first + of + lane * NT; i < p.last; i += 32 * NT) {
-            float x[kVec];
-            unpack_vec<T, kVec>(__ldg(p.vec + i), x);
+    if (own_max != 0 && own_max >= least) t.again[atomicAdd(&t.n_again, 1)] = (uint16_t)tid;
+    team_sync<NT>();
+    // thread by thread of those, vector by vector, dealt out to all threads of the team
+    const int each = (p.last - p.first + NT - 1) / NT, items = t.n_again * each;
+    for (int i0 = tid; i0 < items; i0 += kUnroll * NT) {
+        uint4 raw[kUnroll];
+        int at[kUnroll];
 #pragma unroll
-            for (int k = 0; k < kVec; k++) offer(x[k], p.head + i * kVec + k);
+        for (int k = 0; k < kUnroll; k++) {
+            const int item = i0 + k * NT, which = item / each;
+            at[k] = item < items ? p.first + t.again[which] + (item - which * each) * NT : p.last;
+            if (at[k] < p.last) raw[k] = __ldg(p.vec + at[k]);
         }
-        if (lane == 0 && of < p.loose) {
-            const int i = p.loose_at(of);
-            offer(num_to_float<T>(p.row[i]), i);
+#pragma unroll
+        for (int k = 0; k < kUnroll; k++) {
+            if (at[k] >= p.last) continue;
+            float x[kVec];
+            unpack_vec<T, kVec>(raw[k], x);
+#pragma unroll
+            for (int j = 0; j < kVec; j++) offer(x[j], p.head + at[k] * kVec + j);
         }
     }
+    for (int i = tid; i < p.loose; i += NT) offer(num_to_float<T>(p.row[p.loose_at(i)]), p.loose_at(i));
     team_sync<NT>();
     const int n = t.n_found;
     if (n <= Team<NT>::kCandidates) {
@@ -285,7 +296,7 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT)
     if (tid < p.loose) take_one<ENTROPY>(a, num_to_float<T>(p.row[p.loose_at(tid)]));
     const uint32_t own_max = a.s > 0.f ? rank_bits(a.m) : 0u;  // 0: no entry but -inf (or NaN, where nothing is chosen)
     t.maxima[tid] = own_max;
-    if (tid == 0) t.n_found = 0;
+    if (tid == 0) t.n_found = t.n_again = 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         Stats b;

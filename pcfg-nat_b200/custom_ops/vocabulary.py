@@ -59,6 +59,10 @@ def _on(dev):
     return _STAY if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+def _stream(dev):
+    return torch._C._cuda_getCurrentRawStream(dev.index)  # the handle alone: no object is made for it
+
+
 def _token_tensor(tokens, dev, shape=None):
     if not isinstance(tokens, torch.Tensor) or tokens.dtype != torch.int64 or tokens.device != dev:
         raise RuntimeError(f"tokens must be an int64 tensor on {dev}")
@@ -130,15 +134,14 @@ def _token_logprobs(logits, tokens, top, entropy, ignore, keep):
     tokens = _token_tensor(tokens, dev, shape)
     n = tokens.numel()
     with _on(dev):
-        new = lambda *more, dtype=torch.float32: torch.empty(shape + more, dtype=dtype, device=dev)
-        logprob = new()
-        ent = new() if entropy else None
-        top_lp, top_ix = (new(top), new(top, dtype=torch.int64)) if top else (None, None)
-        kept = new(2) if keep else None
+        logprob = tokens.new_empty(shape, dtype=torch.float32)
+        ent = torch.empty_like(logprob) if entropy else None
+        top_lp, top_ix = (logprob.new_empty(shape + (top,)), tokens.new_empty(shape + (top,))) if top else (None, None)
+        kept = logprob.new_empty(shape + (2,)) if keep else None
         ptr = lambda t: t.data_ptr() if t is not None else None
         rc = _cabi.lib().pcfgnat_token_logprobs(logits.data_ptr(), dt, n, inner, stride_outer, stride_inner, logits.shape[-1],
                                                 tokens.data_ptr(), *ignore, top, logprob.data_ptr(), ptr(ent), ptr(top_lp),
-                                                ptr(top_ix), ptr(kept), _status_of(dev), _ops._stream(dev))
+                                                ptr(top_ix), ptr(kept), _status_of(dev), _stream(dev))
     _cabi.check(rc, "pcfgnat_token_logprobs")
     return logprob, ent, top_lp, top_ix, kept
 
@@ -172,11 +175,11 @@ class TokenLogprobsFunc(Function):
         g_logprob, g_entropy, g_top = cont(g_logprob), cont(g_entropy), cont(g_top)
         ptr = lambda t: t.data_ptr() if t is not None else None
         with _on(dev):
-            d = torch.empty(logits.shape[:-1] + (pitch,), dtype=logits.dtype, device=dev)
+            d = logits.new_empty(logits.shape[:-1] + (pitch,))
             rc = _cabi.lib().pcfgnat_token_logprobs_backward(
                 logits.data_ptr(), _DTYPES[logits.dtype], n, inner, stride_outer, stride_inner, V, tokens.data_ptr(), *ctx.ignore,
                 ctx.top if g_top is not None else 0, kept.data_ptr(), ptr(ent), ptr(top_ix), ptr(g_logprob), ptr(g_entropy),
-                ptr(g_top), d.data_ptr(), pitch, _status_of(dev), _ops._stream(dev))
+                ptr(g_top), d.data_ptr(), pitch, _status_of(dev), _stream(dev))
         _cabi.check(rc, "pcfgnat_token_logprobs_backward")
         return d if pitch == V else d[..., :V], None, None, None, None
 
@@ -224,9 +227,9 @@ def _embed(weight, tokens, scale):
     tokens = _token_tensor(tokens, dev)
     V, H = weight.shape
     with _on(dev):
-        out = torch.empty(tokens.shape + (H,), dtype=weight.dtype, device=dev)
+        out = weight.new_empty(tokens.shape + (H,))
         rc = _cabi.lib().pcfgnat_embed(weight.data_ptr(), dt, weight.stride(0), V, H, tokens.data_ptr(), tokens.numel(), scale,
-                                       out.data_ptr(), _status_of(dev), _ops._stream(dev))
+                                       out.data_ptr(), _status_of(dev), _stream(dev))
     _cabi.check(rc, "pcfgnat_embed")
     return out
 
@@ -243,10 +246,10 @@ def _embed_backward(grad_out, tokens, d_weight, scale, padding, accumulate):
     lib = _cabi.lib()
     nbytes = lib.pcfgnat_embed_backward_workspace_bytes(n, V, H)
     with _on(dev):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws = tokens.new_empty(nbytes, dtype=torch.uint8)
         rc = lib.pcfgnat_embed_backward(g.data_ptr(), dt, rows[2], tokens.data_ptr(), n, V, H, scale, *padding, d_weight.data_ptr(),
                                         _DTYPES[d_weight.dtype], max(d_weight.stride(0), H), int(accumulate), ws.data_ptr(), nbytes,
-                                        _status_of(dev), _ops._stream(dev))
+                                        _status_of(dev), _stream(dev))
     _cabi.check(rc, "pcfgnat_embed_backward")
     return d_weight
 
@@ -265,7 +268,7 @@ class EmbedTokensFunc(Function):
             return None, None, None, None
         (tokens,) = ctx.saved_tensors
         with _on(grad_out.device):
-            d = torch.empty(ctx.table, dtype=grad_out.dtype, device=grad_out.device)
+            d = grad_out.new_empty(ctx.table)
         return _embed_backward(grad_out, tokens.contiguous(), d, ctx.scale, ctx.padding, False), None, None, None
 
 
@@ -375,7 +378,7 @@ def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
         rc = lib.pcfgnat_clip_grad_norm(n, head(src), head(src_kind), head(dst), head(dst_kind), head(numel), max_norm, grad_scale,
-                                        ws.data_ptr(), nbytes, norm.data_ptr(), _ops._stream(dev))
+                                        ws.data_ptr(), nbytes, norm.data_ptr(), _stream(dev))
     if rc == _cabi.ERR_INVALID_ARGUMENT:
         raise RuntimeError("the outputs must not overlap one another or another gradient")
     _cabi.check(rc, "pcfgnat_clip_grad_norm")
