@@ -2,8 +2,8 @@
 //
 // Forward: out[i] = scale * w[token_i].  One read of the rows that occur and one write; a thread moves one vector.
 // Gradient: dw[v] = scale * sum of g[i] over token_i = v, summed in float32 in an order that the input alone decides:
-//   1. embed_sort_kernel  — the positions sorted by token, equal tokens by position.  A block owns a range of the table's rows
-//      and reads all tokens: those below its range count where its entries begin, so no block waits for another.
+//   1. embed_sort_kernel  — the positions grouped by token, equal tokens by position.  A block owns every 128th token of the
+//      table and reads all positions: those of the blocks before it count where its entries begin, so no block waits for another.
 //   2. embed_sum_kernel   — the sorted list cut into pieces of equal length.  A run of one token inside a piece is written
 //      to the table at once; the part of a run that crosses a piece's border goes to scratch memory.
 //   3. embed_join_kernel  — adds up the parts of every run that crosses pieces, in an order that its pieces decide.
@@ -46,18 +46,8 @@ __global__ void __launch_bounds__(kThreads)
 // ---- gradient
 
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kMaxRange = 512;   // rows of the table that one block may own
-constexpr int kAhead = 8;        // loads of 32 tokens that a warp has in flight
-
-__device__ __forceinline__ void zero_row(char *p, int bytes, int lane) {
-    if (!((reinterpret_cast<uintptr_t>(p) | (unsigned)bytes) & 15)) {
-        for (int i = lane; i < bytes / 16; i += 32) reinterpret_cast<uint4 *>(p)[i] = make_uint4(0, 0, 0, 0);
-    } else if (!((reinterpret_cast<uintptr_t>(p) | (unsigned)bytes) & 3)) {
-        for (int i = lane; i < bytes / 4; i += 32) reinterpret_cast<uint32_t *>(p)[i] = 0;
-    } else {
-        for (int i = lane; i < bytes / 2; i += 32) reinterpret_cast<uint16_t *>(p)[i] = 0;
-    }
-}
+constexpr int kMaxRange = 512;   // tokens that one block may own
+constexpr int kAhead = 8;        // loads of a lane in flight
 
 struct Sorted {
     int *token, *at;  // the tokens that count and their positions, by token and then by position
@@ -65,51 +55,81 @@ struct Sorted {
     int *total;       // entries
 };
 
-// Rows of dw without a token are set to zero where `zero`.
-__global__ void __launch_bounds__(kSortThreads)
-    embed_sort_kernel(const int64_t *__restrict__ tokens, int n, int V, int has_padding, int64_t padding, int range, Sorted sorted,
-                      char *dw, int row_bytes, int64_t dw_stride_bytes, int zero, int *status) {
-    extern __shared__ int cell[];  // [warp][row of the range]: tokens of the warp's span, then where the next one goes
+// The whole table set to zero by the blocks behind the sorting ones: those wait for their loads most of the time.
+__device__ void zero_table(char *dw, int64_t rows, int64_t row_bytes, int64_t stride_bytes, int64_t block, int64_t blocks) {
+    const int lane = threadIdx.x & 31;
+    if (stride_bytes == row_bytes) row_bytes *= rows, stride_bytes = 0, rows = 1;  // one long row
+    const bool wide = !((reinterpret_cast<uintptr_t>(dw) | row_bytes | stride_bytes) & 15);
+    if (rows == 1) {
+        const int64_t head = wide ? 0 : min((int64_t)(-reinterpret_cast<uintptr_t>(dw) & 15), row_bytes), vecs = (row_bytes - head) / 16;
+        for (int64_t i = block * kSortThreads + threadIdx.x; i < vecs; i += blocks * kSortThreads)
+            reinterpret_cast<uint4 *>(dw + head)[i] = make_uint4(0, 0, 0, 0);
+        if (block == 0) {
+            const int64_t loose = (row_bytes - vecs * 16) / 2, i = threadIdx.x;  // in units of two bytes
+            if (i < loose) *reinterpret_cast<uint16_t *>(dw + (2 * i < head ? 2 * i : 2 * i + vecs * 16)) = 0;
+        }
+        return;
+    }
+    for (int64_t r = block * kSortWarps + (threadIdx.x >> 5); r < rows; r += blocks * kSortWarps) {
+        char *p = dw + r * stride_bytes;
+        if (wide) {
+            for (int64_t i = lane; i < row_bytes / 16; i += 32) reinterpret_cast<uint4 *>(p)[i] = make_uint4(0, 0, 0, 0);
+        } else {
+            for (int64_t i = lane; i < row_bytes / 2; i += 32) reinterpret_cast<uint16_t *>(p)[i] = 0;
+        }
+    }
+}
+
+// Block b of 2^bits owns the tokens v with v mod 2^bits = b, so that neighbouring (frequent) words are dealt out.
+__global__ void __launch_bounds__(kSortThreads, 2)
+    embed_sort_kernel(const int64_t *__restrict__ tokens, int n, int V, uint32_t padding, int bits, int range, Sorted sorted,
+                      char *dw, int row_bytes, int64_t dw_stride_bytes, int *status) {
+    extern __shared__ int cell[];  // [warp][token of the block]: tokens of the warp's span, then where the next one goes
     __shared__ int warp_sum[kSortWarps], warp_below[kSortWarps];
-    __shared__ int counts[kMaxRange];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int v0 = blockIdx.x * range, rows = min(range, V - v0);
+    const int buckets = 1 << bits;
+    if (blockIdx.x >= buckets) {
+        zero_table(dw, V, row_bytes, dw_stride_bytes, blockIdx.x - buckets, gridDim.x - buckets);
+        return;
+    }
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bucket = blockIdx.x;
     for (int i = tid; i < kSortWarps * range; i += kSortThreads) cell[i] = 0;
     __syncthreads();
     const int span = ((n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
     const int first = (int)min((int64_t)warp * span, (int64_t)n), last = (int)min((int64_t)first + span, (int64_t)n);
     int *mine = cell + warp * range;
-    // the token at i, or -1 where it does not count
-    const auto counted = [&](int64_t t) { return t < 0 || t >= V || (has_padding && t == padding) ? -1 : (int)t; };
+    const uint2 *words = reinterpret_cast<const uint2 *>(tokens);
+    constexpr uint32_t kNone = 0xffffffffu;
+    // the token of a position, kNone where it does not count
+    const auto counted = [&](uint2 t) { return t.y == 0 && t.x < (uint32_t)V && t.x != padding ? t.x : kNone; };
     int below = 0;
     bool bad = false;
-    uint64_t seen = 0;  // groups of 32 of the first 64 that hold tokens of the range; later groups are all looked at again
+    uint64_t seen = 0;  // groups of 32 of the first 64 that hold tokens of the block; later groups are all looked at again
     int group = 0;
     for (int i0 = first; i0 < last; i0 += 32 * kAhead) {
-        int64_t t[kAhead];
+        uint2 t[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; k++) {
             const int i = i0 + k * 32 + lane;
-            t[k] = i < last ? tokens[i] : (int64_t)V;
-            if (i < last && (t[k] < 0 || t[k] >= V)) bad = true;
+            t[k] = i < last ? words[i] : make_uint2(padding, 0);
+            if (bucket == 0 && i < last) bad |= t[k].y != 0 || t[k].x >= (uint32_t)V;
         }
 #pragma unroll
         for (int k = 0; k < kAhead; k++) {
-            const int v = counted(t[k]);
-            const bool in = v >= v0 && v < v0 + rows;
-            below += v >= 0 && v < v0;
-            if (in) atomicAdd(mine + (v - v0), 1);
-            if (__any_sync(0xffffffffu, in) && group < 64) seen |= 1ull << group;
+            const uint32_t v = counted(t[k]);
+            const int of = v == kNone ? buckets : (int)(v & (buckets - 1));
+            below += of < bucket;
+            if (of == bucket) atomicAdd(mine + (v >> bits), 1);
+            if (__any_sync(0xffffffffu, of == bucket) && group < 64) seen |= 1ull << group;
             group++;
         }
     }
-    if (bad && blockIdx.x == 0) flag(status, PCFGNAT_STATUS_BAD_INDEX);
+    if (bad) flag(status, PCFGNAT_STATUS_BAD_INDEX);
     below = __reduce_add_sync(0xffffffffu, below);
     if (lane == 0) warp_below[warp] = below;
     __syncthreads();
-    // where every row of the range begins, and within it every warp
+    // where every token of the block begins, and within it every warp
     int mine_total = 0;
-    if (tid < rows)
+    if (tid < range)
         for (int w = 0; w < kSortWarps; w++) mine_total += cell[w * range + tid];
     int scan = mine_total;
 #pragma unroll
@@ -118,45 +138,48 @@ __global__ void __launch_bounds__(kSortThreads)
         if (lane >= o) scan += x;
     }
     if (lane == 31) warp_sum[warp] = scan;
-    if (tid < kMaxRange) counts[tid] = mine_total;
     __syncthreads();
-    if (tid < rows) {
+    if (tid < range) {
         int next = scan - mine_total;
         for (int w = 0; w < kSortWarps; w++) next += warp_below[w] + (w < warp ? warp_sum[w] : 0);
+#pragma unroll 8
         for (int w = 0; w < kSortWarps; w++) {
             const int c = cell[w * range + tid];
             cell[w * range + tid] = next;
             next += c;
         }
-        sorted.row_end[v0 + tid] = next;
-        if (v0 + tid == V - 1) *sorted.total = next;
+        const int64_t v = ((int64_t)tid << bits) + bucket;
+        if (v < V) sorted.row_end[v] = next;
+        if (tid == range - 1 && bucket == buckets - 1) *sorted.total = next;
     }
     __syncthreads();
-    if (zero)
-        for (int r = warp; r < rows; r += kSortWarps)
-            if (counts[r] == 0) zero_row(dw + (v0 + r) * dw_stride_bytes, row_bytes, lane);
     group = 0;
     for (int i0 = first; i0 < last; i0 += 32 * kAhead, group += kAhead) {
         const uint32_t some = group < 64 ? (uint32_t)(seen >> group) & ((1u << kAhead) - 1) : (1u << kAhead) - 1;
         if (!some) continue;
-        int v[kAhead];
+        uint32_t v[kAhead];
 #pragma unroll
         for (int k = 0; k < kAhead; k++) {
             const int i = i0 + k * 32 + lane;
-            v[k] = (some >> k & 1) && i < last ? counted(tokens[i]) : -1;
+            v[k] = (some >> k & 1) && i < last ? counted(words[i]) : kNone;
         }
 #pragma unroll
         for (int k = 0; k < kAhead; k++) {
-            if (!(some >> k & 1)) continue;
-            const bool in = v[k] >= v0 && v[k] < v0 + rows;
-            const int row = in ? v[k] - v0 : -1;
-            const uint32_t same = __match_any_sync(0xffffffffu, row);
-            int at = 0;
-            if (in) at = mine[row] + __popc(same & ((1u << lane) - 1));
-            __syncwarp();
-            if (in && lane == __ffs(same) - 1) mine[row] += __popc(same);
-            __syncwarp();
-            if (in) sorted.token[at] = v[k], sorted.at[at] = i0 + k * 32 + lane;
+            // one token after the other, as few of them are the block's
+            uint32_t todo = __ballot_sync(0xffffffffu, v[k] != kNone && (int)(v[k] & (buckets - 1)) == bucket);
+            while (todo) {
+                const uint32_t one = __shfl_sync(0xffffffffu, v[k], __ffs(todo) - 1);
+                const uint32_t same = __ballot_sync(0xffffffffu, v[k] == one);
+                const int row = (int)(one >> bits), from = mine[row];
+                __syncwarp();
+                if (v[k] == one) {
+                    const int at = from + __popc(same & ((1u << lane) - 1));
+                    sorted.token[at] = (int)one, sorted.at[at] = i0 + k * 32 + lane;
+                }
+                if (lane == 0) mine[row] = from + __popc(same);
+                __syncwarp();
+                todo &= ~same;
+            }
         }
     }
 }
@@ -362,14 +385,16 @@ int launch_embed_backward(const void *grad, int dtype, int64_t g_stride, const i
                         reinterpret_cast<int *>(ws + 16 + 2 * list), reinterpret_cast<int *>(ws)};
     float *parts = reinterpret_cast<float *>(ws + 16 + 2 * list + round16((size_t)V * sizeof(int)));
     const size_t dw_size = dw_dtype == PCFGNAT_DTYPE_F32 ? 4 : 2;
-    const int64_t per_sm = (V + sm_count() - 1) / sm_count();
-    const int range = (int)(per_sm < kMaxRange ? per_sm : kMaxRange);
+    int bits = 7;  // 128 blocks: as many as one of 1 024 threads each per SM gives
+    while ((V + (1ll << bits) - 1) >> bits > kMaxRange) bits++;
+    const int range = (int)((V + (1ll << bits) - 1) >> bits);
     const size_t smem = (size_t)kSortWarps * range * sizeof(int);
     cudaError_t e = ensure_dynamic_smem(embed_sort_kernel, smem);
     if (e != cudaSuccess) return PCFGNAT_ERR_CUDA;
-    embed_sort_kernel<<<(unsigned)((V + range - 1) / range), kSortThreads, smem, st>>>(
-        tokens, (int)n, (int)V, has_padding, padding, range, sorted, static_cast<char *>(dw), (int)(H * dw_size),
-        (int64_t)(dw_stride * dw_size), !accumulate, status);
+    const uint32_t skip = has_padding && padding >= 0 && padding < V ? (uint32_t)padding : 0xffffffffu;
+    embed_sort_kernel<<<(1u << bits) + (accumulate ? 0u : (unsigned)sm_count()), kSortThreads, smem, st>>>(
+        tokens, (int)n, (int)V, skip, bits, range, sorted, static_cast<char *>(dw), (int)(H * dw_size), (int64_t)(dw_stride * dw_size),
+        status);
     e = cudaGetLastError();
     if (e != cudaSuccess || n == 0) return cuda_rc(e);
     const Pieces p{sorted, parts, warp_entries(n)};
