@@ -33,13 +33,22 @@ __global__ void __launch_bounds__(kThreads)
     const float factor = bad ? CUDART_NAN_F : scale;
     const Raw *from = reinterpret_cast<const Raw *>(weight + (bad ? 0 : t) * w_stride);
     Raw *to = reinterpret_cast<Raw *>(out + r * H);
-#pragma unroll 4
-    for (int c = lane; c < H / VEC; c += lanes) {
-        float x[VEC];
-        unpack_vec<T, VEC>(__ldg(from + c), x);
+    constexpr int kLoads = VEC * sizeof(T) >= 8 ? 4 : 8;  // of a lane in flight
+    const int chunks = H / VEC;
+    for (int c0 = lane; c0 < chunks; c0 += kLoads * lanes) {
+        Raw raw[kLoads];
 #pragma unroll
-        for (int k = 0; k < VEC; k++) x[k] *= factor;
-        to[c] = pack_vec<T, VEC>(x);
+        for (int j = 0; j < kLoads; j++)
+            if (c0 + j * lanes < chunks) raw[j] = __ldg(from + c0 + j * lanes);
+#pragma unroll
+        for (int j = 0; j < kLoads; j++) {
+            if (c0 + j * lanes >= chunks) break;
+            float x[VEC];
+            unpack_vec<T, VEC>(raw[j], x);
+#pragma unroll
+            for (int k = 0; k < VEC; k++) x[k] *= factor;
+            to[c0 + j * lanes] = pack_vec<T, VEC>(x);
+        }
     }
 }
 
@@ -92,6 +101,7 @@ __global__ void __launch_bounds__(kSortThreads, 2)
         return;
     }
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bucket = blockIdx.x;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the next kernel waits for this one's end all the same
     for (int i = tid; i < kSortWarps * range; i += kSortThreads) cell[i] = 0;
     __syncthreads();
     const int span = ((n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
@@ -184,8 +194,24 @@ __global__ void __launch_bounds__(kSortThreads, 2)
     }
 }
 
+// A finished sum into the table.  Every number of the table gets at most one sum per call, so adding to a float32 table by a
+// reduction (which needs not wait for what is there) has one order only.
 template <typename T, int VEC>
 __device__ __forceinline__ void write_row(T *p, const float (&acc)[VEC], float scale, int accumulate) {
+    if constexpr (sizeof(T) == 4) {
+        if (accumulate) {
+            if constexpr (VEC % 4 == 0) {
+#pragma unroll
+                for (int k = 0; k < VEC; k += 4)
+                    atomicAdd(reinterpret_cast<float4 *>(p + k),
+                              make_float4(acc[k] * scale, acc[k + 1] * scale, acc[k + 2] * scale, acc[k + 3] * scale));
+            } else {
+#pragma unroll
+                for (int k = 0; k < VEC; k++) atomicAdd(p + k, acc[k] * scale);
+            }
+            return;
+        }
+    }
     constexpr int kStep = VEC * sizeof(T) > 16 ? 16 / sizeof(T) : VEC;  // numbers of one store
     using Raw = typename RawVec<kStep * sizeof(T)>::type;
 #pragma unroll
@@ -206,17 +232,20 @@ struct Pieces {
     int length;    // entries of a warp, kSumWarps warps to a piece
 };
 
-// A block adds up a piece of the list for 32 * VEC columns, a warp an equal share of it, a lane VEC columns.  A warp's runs that
-// cross its borders are joined in shared memory, in the list's order, and so are given on only where they cross the piece's.
-template <typename G, typename W, int VEC>
+// A block adds up a piece of the list for a tile of columns, a warp an equal share of it, a lane REP times VEC columns (32 * VEC
+// apart).  A warp's runs that cross its borders are joined in shared memory, in the list's order, and so are given on only where
+// they cross the piece's.
+template <typename G, typename W, int VEC, int REP>
 __global__ void __launch_bounds__(32 * kSumWarps)
     embed_sum_kernel(const G *__restrict__ grad, int64_t g_stride, int H, Pieces p, W *dw, int64_t dw_stride, float scale,
                      int accumulate) {
     using Raw = typename RawVec<VEC * sizeof(G)>::type;
-    __shared__ float crossing[kSumWarps][2][32 * VEC];
+    constexpr int kTile = 32 * VEC * REP;
+    __shared__ float crossing[kSumWarps][2][kTile];
+    __shared__ int4 ends[kSumWarps];  // of a warp's share: first and last token, whether those runs go on before and behind it
+    chain_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c = (blockIdx.y * 32 + lane) * VEC;
-    const bool there = c < H;
+    const int tile = blockIdx.y * kTile, c = tile + lane * VEC;  // of the lane's columns, the first
     const int total = *p.sorted.total;
     const int64_t begin64 = ((int64_t)blockIdx.x * kSumWarps + warp) * p.length;
     const int *token = p.sorted.token;
@@ -224,63 +253,70 @@ __global__ void __launch_bounds__(32 * kSumWarps)
     if (begin64 < total) {
         const int begin = (int)begin64, end = min(begin + p.length, total);
         const int before = begin > 0 ? token[begin - 1] : -1, after = end < total ? token[end] : -1;
-        float acc[VEC] = {};
+        float acc[REP][VEC] = {};
         int run = token[begin];
         bool began_before = run == before;
+        if (lane == 0) {
+            const int tail = token[end - 1];
+            ends[warp] = make_int4(run, tail, run == before, tail == after);
+        }
         for (int i0 = begin; i0 < end; i0 += 32) {
             const int count = min(32, end - i0);
             const int my_token = lane < count ? token[i0 + lane] : -1, my_at = lane < count ? p.sorted.at[i0 + lane] : 0;
             const int behind = i0 + count < end ? token[i0 + count] : -1;
             for (int j0 = 0; j0 < count; j0 += kAhead) {
-                Raw raw[kAhead];
+                Raw raw[kAhead][REP];
 #pragma unroll
                 for (int j = 0; j < kAhead; j++) {
-                    const int at = __shfl_sync(0xffffffffu, my_at, (j0 + j) & 31);
-                    if (there && j0 + j < count) raw[j] = __ldg(reinterpret_cast<const Raw *>(grad + at * g_stride + c));
+                    const G *row = grad + __shfl_sync(0xffffffffu, my_at, (j0 + j) & 31) * g_stride;
+#pragma unroll
+                    for (int q = 0; q < REP; q++)
+                        if (j0 + j < count && c + q * 32 * VEC < H) raw[j][q] = __ldg(reinterpret_cast<const Raw *>(row + c + q * 32 * VEC));
                 }
 #pragma unroll
                 for (int j = 0; j < kAhead; j++) {
                     const int next_of = __shfl_sync(0xffffffffu, my_token, (j0 + j + 1) & 31);
-                    if (j0 + j < count) {  // the same for the whole warp
+                    if (j0 + j >= count) continue;  // the same for the whole warp
+#pragma unroll
+                    for (int q = 0; q < REP; q++) {
                         float x[VEC];
-                        unpack_vec<G, VEC>(raw[j], x);
+                        unpack_vec<G, VEC>(raw[j][q], x);
 #pragma unroll
-                        for (int k = 0; k < VEC; k++) acc[k] += x[k];
-                        const bool last = j0 + j + 1 == count;
-                        const int next = last ? behind : next_of;
-                        if (next != run) {
-                            const bool goes_on = next < 0 && run == after;
-                            if (began_before || goes_on) {
-                                float *to = crossing[warp][began_before ? 0 : 1] + lane * VEC;
-#pragma unroll
-                                for (int k = 0; k < VEC; k++) to[k] = acc[k];
-                            } else if (there) {
-                                write_row<W, VEC>(dw + run * dw_stride + c, acc, scale, accumulate);
-                            }
-#pragma unroll
-                            for (int k = 0; k < VEC; k++) acc[k] = 0.f;
-                            run = next;
-                            began_before = false;
-                        }
+                        for (int k = 0; k < VEC; k++) acc[q][k] += x[k];
                     }
+                    const int next = j0 + j + 1 == count ? behind : next_of;
+                    if (next == run) continue;
+                    const bool goes_on = next < 0 && run == after;
+#pragma unroll
+                    for (int q = 0; q < REP; q++) {
+                        if (began_before || goes_on) {
+                            float *to = crossing[warp][began_before ? 0 : 1] + q * 32 * VEC + lane * VEC;
+#pragma unroll
+                            for (int k = 0; k < VEC; k++) to[k] = acc[q][k];
+                        } else if (c + q * 32 * VEC < H) {
+                            write_row<W, VEC>(dw + run * dw_stride + c + q * 32 * VEC, acc[q], scale, accumulate);
+                        }
+#pragma unroll
+                        for (int k = 0; k < VEC; k++) acc[q][k] = 0.f;
+                    }
+                    run = next;
+                    began_before = false;
                 }
             }
         }
     }
     __syncthreads();
-    // 32 * VEC columns by as many threads: what the warps left, in the list's order
-    for (int col = threadIdx.x; col < 32 * VEC; col += 32 * kSumWarps) {
-        const int cc = blockIdx.y * 32 * VEC + col;
+    // a thread per column: what the warps left, in the list's order
+    for (int col = threadIdx.x; col < kTile; col += 32 * kSumWarps) {
+        const int cc = tile + col;
         if (cc >= H) continue;
         float *give = p.parts + (int64_t)blockIdx.x * 2 * H + cc;
         float acc[1] = {0.f};
         bool from_outside = false, open = false;
         for (int w = 0; w < kSumWarps; w++) {
-            const int64_t b64 = ((int64_t)blockIdx.x * kSumWarps + w) * p.length;
-            if (b64 >= total) break;
-            const int b = (int)b64, e = min(b + p.length, total);
-            const int head = token[b], tail = token[e - 1];
-            const bool before = b > 0 && token[b - 1] == head, behind = e < total && token[e] == tail;
+            if (((int64_t)blockIdx.x * kSumWarps + w) * p.length >= total) break;
+            const int head = ends[w].x, tail = ends[w].y;
+            const bool before = ends[w].z, behind = ends[w].w;
             if (before) {
                 if (w == 0) from_outside = true;
                 acc[0] += crossing[w][0][col];
@@ -298,30 +334,42 @@ __global__ void __launch_bounds__(32 * kSumWarps)
     }
 }
 
-// The runs that cross pieces: the first part, and those of the pieces behind it in eight sums of every eighth one.
+constexpr int kJoinGroups = 16, kJoinColumns = 128;
+
+// The runs that cross pieces: the first part and those of the pieces behind it, sixteen warps taking every sixteenth piece, a
+// lane four columns.
 template <typename W>
-__global__ void __launch_bounds__(kThreads) embed_join_kernel(int H, Pieces p, W *dw, int64_t dw_stride, float scale, int accumulate) {
-    __shared__ float sums[8][33];
+__global__ void __launch_bounds__(32 * kJoinGroups)
+    embed_join_kernel(int H, Pieces p, W *dw, int64_t dw_stride, float scale, int accumulate) {
+    __shared__ float sums[kJoinGroups][kJoinColumns];
+    chain_begin();
     const int total = *p.sorted.total, length = p.length * kSumWarps;
     const int64_t begin64 = (int64_t)blockIdx.x * length;
     if (begin64 + length >= total) return;
     const int begin = (int)begin64, end = begin + length;
-    const int token = p.sorted.token[end - 1];
-    if (p.sorted.token[end] != token || (begin > 0 && p.sorted.token[begin - 1] == token)) return;
+    const int token = p.sorted.token[end - 1], behind = p.sorted.token[end], before = begin > 0 ? p.sorted.token[begin - 1] : -1;
+    if (behind != token || before == token) return;
     const int last = (p.sorted.row_end[token] - 1) / length;  // the piece in which the run ends
-    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, c = blockIdx.y * 32 + lane;
-    float acc = 0.f;
-    if (c < H) {
-        if (group == 0) acc = p.parts[(int64_t)blockIdx.x * 2 * H + H + c];
-#pragma unroll 8
-        for (int64_t q = (int64_t)blockIdx.x + 1 + group; q <= last; q += 8) acc += p.parts[q * 2 * H + c];
-    }
-    sums[group][lane] = acc;
+    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, tile = blockIdx.y * kJoinColumns;
+    float acc[4] = {};
+    const auto add = [&](int64_t piece, int which) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int c = tile + k * 32 + lane;
+            if (c < H) acc[k] += p.parts[(piece * 2 + which) * H + c];
+        }
+    };
+    if (group == 0) add(blockIdx.x, 1);
+#pragma unroll 4
+    for (int q = (int)blockIdx.x + 1 + group; q <= last; q += kJoinGroups) add(q, 0);
+#pragma unroll
+    for (int k = 0; k < 4; k++) sums[group][k * 32 + lane] = acc[k];
     __syncthreads();
-    if (group == 0 && c < H) {
+    const int col = threadIdx.x, c = tile + col;
+    if (col < kJoinColumns && c < H) {
         float sum[1] = {0.f};
 #pragma unroll
-        for (int g = 0; g < 8; g++) sum[0] += sums[g][lane];
+        for (int g = 0; g < kJoinGroups; g++) sum[0] += sums[g][col];
         write_row<W, 1>(dw + token * dw_stride + c, sum, scale, accumulate);
     }
 }
@@ -409,18 +457,35 @@ int launch_embed_backward(const void *grad, int dtype, int64_t g_stride, const i
             };
             const int wide_g = widest(bits(grad, g_stride, sizeof(G)), sizeof(G)) / (int)sizeof(G);
             const int wide_w = widest(bits(dw, dw_stride, sizeof(W)), sizeof(W)) / (int)sizeof(W);
-            const auto sum = [&](auto vec) {
-                constexpr int VEC = decltype(vec)::value;
-                embed_sum_kernel<G, W, VEC><<<dim3(pieces, (unsigned)((H / VEC + 31) / 32)), 32 * kSumWarps, 0, st>>>(
-                    static_cast<const G *>(grad), g_stride, H, p, static_cast<W *>(dw), dw_stride, scale, accumulate);
+            // every kernel waits for the one before it to end, but may be scheduled before that
+            const auto launch = [&](auto kernel, unsigned tiles, unsigned threads, auto... args) {
+                cudaLaunchConfig_t cfg = {};
+                cfg.gridDim = dim3(pieces, tiles);
+                cfg.blockDim = dim3(threads);
+                cfg.stream = st;
+                cudaLaunchAttribute attr[1];
+                attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+                attr[0].val.programmaticStreamSerializationAllowed = 1;
+                cfg.attrs = attr;
+                cfg.numAttrs = 1;
+                return cudaLaunchKernelEx(&cfg, kernel, args...);
+            };
+            const auto sum = [&](auto vec, auto rep) {
+                constexpr int VEC = decltype(vec)::value, REP = decltype(rep)::value;
+                return launch(embed_sum_kernel<G, W, VEC, REP>, (unsigned)((H + 32 * VEC * REP - 1) / (32 * VEC * REP)), 32 * kSumWarps,
+                              static_cast<const G *>(grad), g_stride, H, p, static_cast<W *>(dw), dw_stride, scale, accumulate);
             };
             constexpr int kWide = 16 / sizeof(G), kWideW = 16 / sizeof(W) < kWide ? 16 / sizeof(W) : kWide;
-            if (wide_g >= kWide && wide_w >= kWideW && H % kWide == 0) sum(std::integral_constant<int, kWide>());
-            else if (wide_g >= 2 && wide_w >= 2) sum(std::integral_constant<int, 2>());
-            else sum(std::integral_constant<int, 1>());
+            using std::integral_constant;
+            cudaError_t rc;
+            if (wide_g >= kWide && wide_w >= kWideW && H % kWide == 0) rc = sum(integral_constant<int, kWide>(), integral_constant<int, 1>());
+            else if (wide_g >= 2 && wide_w >= 2) rc = sum(integral_constant<int, 2>(), integral_constant<int, 2>());
+            else rc = sum(integral_constant<int, 1>(), integral_constant<int, 4>());
+            if (rc != cudaSuccess) return (int)PCFGNAT_ERR_CUDA;
             if (pieces > 1)  // one piece has no border
-                embed_join_kernel<W><<<dim3(pieces, (unsigned)((H + 31) / 32)), kThreads, 0, st>>>(H, p, static_cast<W *>(dw), dw_stride,
-                                                                                             scale, accumulate);
+                rc = launch(embed_join_kernel<W>, (unsigned)((H + kJoinColumns - 1) / kJoinColumns), 32 * kJoinGroups, H, p,
+                            static_cast<W *>(dw), dw_stride, scale, accumulate);
+            if (rc != cudaSuccess) return (int)PCFGNAT_ERR_CUDA;
             return cuda_rc(cudaGetLastError());
         };
         if (dw_dtype == PCFGNAT_DTYPE_F32) return run(float());

@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kUnroll = 4;            // 16-byte loads of a thread in flight
 constexpr int kMaxTop = PCFGNAT_MAX_TOP;
+static_assert(kMaxTop <= 32, "a warp writes the alternatives of a row");
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFarBelow = -1.0e4f;  // 2^x of anything smaller is 0, and 0 * x stays 0 (with -inf it would be NaN)
 
@@ -38,12 +39,16 @@ __device__ __forceinline__ void rescale(Stats &a, float m) {
     a.s *= r;
     a.m = m;
 }
-__device__ __forceinline__ Stats join(Stats a, Stats b) {
-    const float m = max_nan(a.m, b.m);
+// The triples of a warp's lanes as one, in every lane: one maximum, one rescaling, two sums.
+__device__ __forceinline__ Stats join_lanes(Stats a) {
+    float m;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(a.m));
     rescale(a, m);
-    rescale(b, m);
-    a.s += b.s;
-    a.u += b.u;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+    }
     return a;
 }
 
@@ -153,33 +158,35 @@ __device__ __forceinline__ void team_sync() {
     else __syncthreads();
 }
 
-// The `top` best entries of a part, sorted, into t.best (0 where there are fewer).
-template <typename T, int NT>
-__device__ void best_entries(Team<NT> &t, const Part<T> &p, int top, uint32_t own_max, int tid) {
-    constexpr int kVec = RowCut<T>::kVec, kWarps = Team<NT>::kWarps;
-    const int warp = tid >> 5, lane = tid & 31;
-    if (warp == 0) {  // the top-th largest of the threads' maxima
-        uint32_t v[kWarps], best = 0, at = 0;
+// The top-th largest of the threads' maxima, by one warp; 0 where fewer threads saw anything: every number is a candidate.
+template <int NT>
+__device__ __forceinline__ uint32_t lower_bound_of_top(const Team<NT> &t, int top, int lane) {
+    constexpr int kWarps = Team<NT>::kWarps;
+    uint32_t v[kWarps], best = 0, at = 0;
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) v[w] = t.maxima[w * 32 + lane], best = max(best, v[w]);
-        for (int k = 0; k < top; k++) {
-            at = __reduce_max_sync(0xffffffffu, best);
-            if (at == 0) break;  // fewer threads than that saw anything: every number is a candidate
-            const uint32_t who = __ballot_sync(0xffffffffu, best == at);
-            if (lane == __ffs(who) - 1) {
-                bool gone = false;
-                best = 0;
+    for (int w = 0; w < kWarps; w++) v[w] = t.maxima[w * 32 + lane], best = max(best, v[w]);
+    for (int k = 0; k < top; k++) {
+        at = __reduce_max_sync(0xffffffffu, best);
+        if (at == 0) break;
+        const uint32_t who = __ballot_sync(0xffffffffu, best == at);
+        if (lane == __ffs(who) - 1) {
+            bool gone = false;
+            best = 0;
 #pragma unroll
-                for (int w = 0; w < kWarps; w++) {
-                    if (!gone && v[w] == at) v[w] = 0, gone = true;
-                    best = max(best, v[w]);
-                }
+            for (int w = 0; w < kWarps; w++) {
+                if (!gone && v[w] == at) v[w] = 0, gone = true;
+                best = max(best, v[w]);
             }
         }
-        if (lane == 0) t.bound = at;
-        if (lane < top) t.best[lane] = 0;
     }
-    team_sync<NT>();
+    return at;
+}
+
+// The `top` best entries of a part, sorted, into t.best (zeroed before; they stay 0 where there are fewer).
+template <typename T, int NT>
+__device__ __forceinline__ void best_entries(Team<NT> &t, const Part<T> &p, int top, uint32_t own_max, int tid) {
+    constexpr int kVec = RowCut<T>::kVec, kWarps = Team<NT>::kWarps;
+    const int warp = tid >> 5, lane = tid & 31;
     const uint32_t least = t.bound;
     const auto offer = [&](float x, int index) {
         if (x == neg_inf() || rank_bits(x) < least) return;
@@ -295,59 +302,51 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT)
     }
     if (tid < p.loose) take_one<ENTROPY>(a, num_to_float<T>(p.row[p.loose_at(tid)]));
     const uint32_t own_max = a.s > 0.f ? rank_bits(a.m) : 0u;  // 0: no entry but -inf (or NaN, where nothing is chosen)
-    t.maxima[tid] = own_max;
-    if (tid == 0) t.n_found = t.n_again = 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Stats b;
-        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-        b.u = __shfl_xor_sync(0xffffffffu, a.u, o);
-        a = join(a, b);
-    }
-    if (Team<NT>::kWarps > 1) {
-        if (lane == 0) t.part[warp] = a;
-        team_sync<NT>();
-        a = t.part[0];
-#pragma unroll
-        for (int w = 1; w < Team<NT>::kWarps; w++) a = join(a, t.part[w]);
-    } else {
-        team_sync<NT>();
+    if (top) t.maxima[tid] = own_max;
+    a = join_lanes(a);
+    if (Team<NT>::kWarps > 1 && lane == 0) t.part[warp] = a;
+    team_sync<NT>();
+    if (warp == 0) {  // the rest is this warp's, but for the alternatives
+        if (Team<NT>::kWarps > 1) a = join_lanes(lane < Team<NT>::kWarps ? t.part[lane] : Stats());
+        if (top) {
+            const uint32_t least = a.s > 0.f ? lower_bound_of_top<NT>(t, top, lane) : 0xffffffffu;  // that many or none
+            if (lane == 0) t.bound = least, t.n_found = t.n_again = 0;
+            t.best[lane] = 0;
+        }
+    } else if (!top && parts == 1) {
+        return;
     }
     if (top) {
-        if (a.s > 0.f) best_entries<T, NT>(t, p, top, own_max, tid);
-        else if (tid < top) t.best[tid] = 0;
+        team_sync<NT>();
+        best_entries<T, NT>(t, p, top, own_max, tid);
+        team_sync<NT>();
     }
-    int n_best = top;
     if (parts > 1) {
         if (tid == 0) t.whole = a;
         cluster.sync();
         if (rank == 0) {
-            for (int q = 1; q < parts; q++) a = join(a, *cluster.map_shared_rank(&t.whole, q));
+            if (warp == 0) a = join_lanes(lane < parts ? *cluster.map_shared_rank(&t.whole, lane) : Stats());
             if (top) {  // the parts' best entries side by side
-                n_best = parts * top;
-                for (int i = tid; i < n_best; i += NT) t.found[i] = cluster.map_shared_rank(t.best, i / top)[i % top];
+                for (int i = tid; i < parts * top; i += NT) t.found[i] = cluster.map_shared_rank(t.best, i / top)[i % top];
                 __syncthreads();
                 if (tid < top) t.best[tid] = 0;
-                __syncthreads();
             }
         }
         cluster.sync();  // a block's memory is there until it has been read
         if (rank) return;
         if (top) {
-            for (int i = tid; i < n_best; i += NT) {
+            for (int i = tid; i < parts * top; i += NT) {
                 const uint64_t key = t.found[i];
                 int better = 0;
-                for (int j = 0; j < n_best; j++) better += t.found[j] > key;
+                for (int j = 0; j < parts * top; j++) better += t.found[j] > key;
                 if (key && better < top) t.best[better] = key;
             }
             __syncthreads();
         }
-    } else if (top) {
-        team_sync<NT>();
     }
+    if (warp) return;
     const float log_s = logf(a.s);  // -inf for a row of nothing but -inf
-    if (tid == 0) {
+    if (lane == 0) {
         float lp;
         if (token < 0 || token >= V) {
             lp = CUDART_NAN_F;
@@ -359,11 +358,11 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT)
         if (ENTROPY) out.entropy[r] = a.s == 0.f ? 0.f : log_s - kLn2 * (a.u / a.s);
         if (out.kept) out.kept[2 * r] = a.m, out.kept[2 * r + 1] = log_s;
     }
-    if (tid < top) {
-        const uint64_t key = a.s > 0.f ? t.best[tid] : 0;
+    if (lane < top) {
+        const uint64_t key = a.s > 0.f ? t.best[lane] : 0;
         // a row that is no distribution is NaN; an alternative that does not exist has no probability
-        out.top_logprob[r * top + tid] = key ? (key_value(key) - a.m) - log_s : a.s >= 0.f ? neg_inf() : CUDART_NAN_F;
-        out.top_index[r * top + tid] = key ? key_index(key) : -1;
+        out.top_logprob[r * top + lane] = key ? (key_value(key) - a.m) - log_s : a.s >= 0.f ? neg_inf() : CUDART_NAN_F;
+        out.top_index[r * top + lane] = key ? key_index(key) : -1;
     }
 }
 
