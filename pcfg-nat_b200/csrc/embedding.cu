@@ -2,12 +2,15 @@
 //
 // Forward: out[i] = scale * w[token_i].  One read of the rows that occur and one write; a thread moves one vector.
 // Gradient: dw[v] = scale * sum of g[i] over token_i = v, summed in float32 in an order that the input alone decides:
-//   1. embed_sort_kernel  — the positions grouped by token, equal tokens by position.  A block owns every 128th token of the
-//      table and reads all positions: those of the blocks before it count where its entries begin, so no block waits for another.
-//   2. embed_sum_kernel   — the sorted list cut into pieces of equal length.  A run of one token inside a piece is written
+//   1. embed_group_kernel — every tile of 1 024 positions grouped by bucket, the token modulo 128, in the positions' order.
+//   2. embed_sort_kernel  — a block per bucket gathers its groups of all tiles and sorts them by token; what the tiles hold of the
+//      buckets before it says where its part of the list begins, so no block waits for another.
+//   3. embed_sum_kernel   — the sorted list cut into pieces of equal length.  A run of one token inside a piece is written
 //      to the table at once; the part of a run that crosses a piece's border goes to scratch memory.
-//   3. embed_join_kernel  — adds up the parts of every run that crosses pieces, in an order that its pieces decide.
+//   4. embed_join_kernel  — adds up the parts of every run that crosses pieces, in an order that its pieces decide.
 // A placeholder that fills most positions is thus spread over as many blocks as its share of the list.
+#include <algorithm>
+
 #include "row_vectors.cuh"
 
 namespace pcfgnat {
@@ -55,23 +58,21 @@ __global__ void __launch_bounds__(kThreads)
 // ---- gradient
 
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kMaxRange = 512;   // tokens that one block may own
-constexpr int kAhead = 8;        // loads of a lane in flight
+constexpr int kTile = 1024;           // positions that one block of the first kernel groups
+constexpr int kBucketBits = 7, kBuckets = 1 << kBucketBits;  // a bucket: the tokens v with the same v mod 128
+constexpr int kMaxRange = 1024;       // tokens of a bucket that are sorted at a time
+constexpr int kBatch = 4;             // entries of a lane in flight
+constexpr int kAhead = 7;             // rows that a warp has in flight
+constexpr int kShare = 8;             // entries of a warp's share are a multiple of it
 
-struct Sorted {
-    int *token, *at;  // the tokens that count and their positions, by token and then by position
-    int *row_end;     // [V] where the list's entries of a token end
-    int *total;       // entries
-};
-
-// The whole table set to zero by the blocks behind the sorting ones: those wait for their loads most of the time.
+// Rows of the table set to zero by the blocks behind the sorting ones, which wait for their loads most of the time.
 __device__ void zero_table(char *dw, int64_t rows, int64_t row_bytes, int64_t stride_bytes, int64_t block, int64_t blocks) {
     const int lane = threadIdx.x & 31;
     if (stride_bytes == row_bytes) row_bytes *= rows, stride_bytes = 0, rows = 1;  // one long row
     const bool wide = !((reinterpret_cast<uintptr_t>(dw) | row_bytes | stride_bytes) & 15);
     if (rows == 1) {
         const int64_t head = wide ? 0 : min((int64_t)(-reinterpret_cast<uintptr_t>(dw) & 15), row_bytes), vecs = (row_bytes - head) / 16;
-        for (int64_t i = block * kSortThreads + threadIdx.x; i < vecs; i += blocks * kSortThreads)
+        for (int64_t i = block * blockDim.x + threadIdx.x; i < vecs; i += blocks * blockDim.x)
             reinterpret_cast<uint4 *>(dw + head)[i] = make_uint4(0, 0, 0, 0);
         if (block == 0) {
             const int64_t loose = (row_bytes - vecs * 16) / 2, i = threadIdx.x;  // in units of two bytes
@@ -79,7 +80,7 @@ __device__ void zero_table(char *dw, int64_t rows, int64_t row_bytes, int64_t st
         }
         return;
     }
-    for (int64_t r = block * kSortWarps + (threadIdx.x >> 5); r < rows; r += blocks * kSortWarps) {
+    for (int64_t r = block * (blockDim.x / 32) + (threadIdx.x >> 5); r < rows; r += blocks * (blockDim.x / 32)) {
         char *p = dw + r * stride_bytes;
         if (wide) {
             for (int64_t i = lane; i < row_bytes / 16; i += 32) reinterpret_cast<uint4 *>(p)[i] = make_uint4(0, 0, 0, 0);
@@ -89,109 +90,230 @@ __device__ void zero_table(char *dw, int64_t rows, int64_t row_bytes, int64_t st
     }
 }
 
-// Block b of 2^bits owns the tokens v with v mod 2^bits = b, so that neighbouring (frequent) words are dealt out.
+struct Sorted {
+    int *token, *at;     // the tokens that count and their positions, equal tokens side by side
+    int *row_end;        // [V] where the list's entries of a token end
+    int *total;          // entries
+    uint2 *grouped;      // [tile][kTile] (token / kBuckets, position) by bucket
+    int *bucket_begin;   // [tile][kBuckets + 1] where a bucket's entries of the tile begin
+};
+
+struct Zeroed {  // rows [first, last) of the table that a launch's further blocks set to zero
+    char *dw;
+    int64_t first, last, row_bytes, stride_bytes;
+    __device__ __forceinline__ void run(int block, int blocks) const {
+        zero_table(dw + first * stride_bytes, last - first, row_bytes, stride_bytes, block, blocks);
+    }
+};
+
+// The positions of a tile grouped by bucket, in their order within one.
+__global__ void __launch_bounds__(kTile, 2)
+    embed_group_kernel(const int64_t *__restrict__ tokens, int n, int V, uint32_t padding, int tiles, Sorted sorted, Zeroed zeroed,
+                       int *status) {
+    __shared__ int cell[kTile / 32][kBuckets];
+    __shared__ int begin[kBuckets], warp_sum[kBuckets / 32];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the next kernel waits for this one's end all the same
+    if ((int)blockIdx.x >= tiles) {
+        zeroed.run(blockIdx.x - tiles, gridDim.x - tiles);
+        return;
+    }
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int64_t i = (int64_t)blockIdx.x * kTile + tid;
+    const uint2 t = i < n ? reinterpret_cast<const uint2 *>(tokens)[i] : make_uint2(padding, 0);
+    const bool inside = t.y == 0 && t.x < (uint32_t)V, counts = inside && t.x != padding;
+    if (i < n && !inside) flag(status, PCFGNAT_STATUS_BAD_INDEX);
+    const int bucket = t.x & (kBuckets - 1);
+    uint32_t same = __ballot_sync(0xffffffffu, counts);  // the lanes with the same bucket
+#pragma unroll
+    for (int k = 0; k < kBucketBits; k++) {
+        const uint32_t set = __ballot_sync(0xffffffffu, bucket >> k & 1);
+        same &= bucket >> k & 1 ? set : ~set;
+    }
+#pragma unroll
+    for (int k = 0; k < kBuckets / 32; k++) cell[warp][k * 32 + lane] = 0;
+    __syncwarp();
+    const int rank = __popc(same & ((1u << lane) - 1));
+    if (counts && rank == 0) cell[warp][bucket] = __popc(same);
+    __syncthreads();
+    if (tid < kBuckets) {
+        int sum = 0;
+#pragma unroll 8
+        for (int w = 0; w < kTile / 32; w++) {
+            const int c = cell[w][tid];
+            cell[w][tid] = sum;
+            sum += c;
+        }
+        int scan = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += x;
+        }
+        if (lane == 31) warp_sum[warp] = scan;
+        begin[tid] = scan - sum;
+    }
+    __syncthreads();
+    if (tid < kBuckets) {
+        int before = begin[tid];
+        for (int w = 0; w < warp; w++) before += warp_sum[w];
+        begin[tid] = before;
+        int *out = sorted.bucket_begin + (int64_t)blockIdx.x * (kBuckets + 1);
+        out[tid] = before;
+        if (tid == 0) {
+            int all = 0;
+            for (int w = 0; w < kBuckets / 32; w++) all += warp_sum[w];
+            out[kBuckets] = all;
+        }
+    }
+    __syncthreads();
+    if (counts)
+        sorted.grouped[(int64_t)blockIdx.x * kTile + begin[bucket] + cell[warp][bucket] + rank] = make_uint2(t.x >> kBucketBits, (uint32_t)i);
+}
+
+// The entries of a bucket in the tiles that one warp goes over, at most one tile per lane, numbered through.
+struct Span {
+    int begin, count, shift;  // of the lane's tile: its first number, its entries, and from a number to the place in the tiles' list
+    int n;
+    // part of parts: where there are fewer tiles than warps, several of them share one.
+    __device__ __forceinline__ Span(const Sorted &s, int bucket, int tile0, int tiles, int part, int parts, int lane, int &below) {
+        int from = 0;
+        count = 0;
+        if (lane < tiles) {
+            const int *b = s.bucket_begin + (int64_t)(tile0 + lane) * (kBuckets + 1) + bucket;
+            from = b[0], count = b[1] - from;
+        }
+        if (part == 0) below += from;
+        const int first = count * part / parts;
+        count = count * (part + 1) / parts - first;
+        from += first;
+        begin = count;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, begin, o);
+            if (lane >= o) begin += x;
+        }
+        n = __shfl_sync(0xffffffffu, begin, 31);
+        begin -= count;
+        shift = lane * kTile + from - begin;
+    }
+    // Entry e of them; e may differ from lane to lane, but all lanes call.
+    __device__ __forceinline__ uint2 entry(const Sorted &s, int tile0, int tiles, int e, uint2 none) const {
+        int of = 0;
+        if (tiles > 1) {
+#pragma unroll
+            for (int step = 16; step > 0; step /= 2)
+                if (__shfl_sync(0xffffffffu, begin, of + step) <= e) of += step;
+        }
+        const int at = __shfl_sync(0xffffffffu, shift, of) + e;
+        return e < n ? s.grouped[(int64_t)tile0 * kTile + at] : none;
+    }
+};
+
+// A block sorts a bucket by token: counted per warp and token, numbered, placed.
 __global__ void __launch_bounds__(kSortThreads, 2)
-    embed_sort_kernel(const int64_t *__restrict__ tokens, int n, int V, uint32_t padding, int bits, int range, Sorted sorted,
-                      char *dw, int row_bytes, int64_t dw_stride_bytes, int *status) {
-    extern __shared__ int cell[];  // [warp][token of the block]: tokens of the warp's span, then where the next one goes
-    __shared__ int warp_sum[kSortWarps], warp_below[kSortWarps];
-    const int buckets = 1 << bits;
-    if (blockIdx.x >= buckets) {
-        zero_table(dw, V, row_bytes, dw_stride_bytes, blockIdx.x - buckets, gridDim.x - buckets);
+    embed_sort_kernel(int V, int tiles, int range, Sorted sorted, Zeroed zeroed) {
+    extern __shared__ int cell[];  // [warp][token of the bucket]: entries of the warp's span, then where the next one goes
+    __shared__ int warp_sum[kSortWarps], base;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (blockIdx.x >= kBuckets) {
+        zeroed.run(blockIdx.x - kBuckets, gridDim.x - kBuckets);
         return;
     }
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bucket = blockIdx.x;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the next kernel waits for this one's end all the same
+    if (tid == 0) base = 0;
     for (int i = tid; i < kSortWarps * range; i += kSortThreads) cell[i] = 0;
     __syncthreads();
-    const int span = ((n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
-    const int first = (int)min((int64_t)warp * span, (int64_t)n), last = (int)min((int64_t)first + span, (int64_t)n);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int tokens = (V - bucket + kBuckets - 1) >> kBucketBits;  // of the bucket (0 where V is smaller than its number)
+    const uint2 none = make_uint2(0xffffffffu, 0);
+    // A warp's tiles lie side by side, at most 32 of them; longer lists are gone over 1 024 tiles at a time.
+    const auto over = [&](auto visit) {
+        int below = 0;
+        for (int chunk = 0; chunk < tiles; chunk += kSortWarps * 32) {
+            const int there = min(kSortWarps * 32, tiles - chunk), each = (there + kSortWarps - 1) / kSortWarps;
+            const int parts = max(1, kSortWarps / there), unit = warp / parts;
+            const int tile0 = min(chunk + unit * each, tiles), mine = min(each, tiles - tile0);
+            const Span span(sorted, bucket, tile0, mine, warp % parts, parts, lane, below);
+            for (int e0 = lane; e0 - lane < span.n; e0 += 32 * kBatch) {
+                uint2 entry[kBatch];
+#pragma unroll
+                for (int k = 0; k < kBatch; k++) entry[k] = span.entry(sorted, tile0, mine, e0 + k * 32, none);
+#pragma unroll
+                for (int k = 0; k < kBatch; k++) visit(entry[k]);
+            }
+        }
+        return below;
+    };
     int *mine = cell + warp * range;
-    const uint2 *words = reinterpret_cast<const uint2 *>(tokens);
-    constexpr uint32_t kNone = 0xffffffffu;
-    // the token of a position, kNone where it does not count
-    const auto counted = [&](uint2 t) { return t.y == 0 && t.x < (uint32_t)V && t.x != padding ? t.x : kNone; };
-    int below = 0;
-    bool bad = false;
-    uint64_t seen = 0;  // groups of 32 of the first 64 that hold tokens of the block; later groups are all looked at again
-    int group = 0;
-    for (int i0 = first; i0 < last; i0 += 32 * kAhead) {
-        uint2 t[kAhead];
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            const int i = i0 + k * 32 + lane;
-            t[k] = i < last ? words[i] : make_uint2(padding, 0);
-            if (bucket == 0 && i < last) bad |= t[k].y != 0 || t[k].x >= (uint32_t)V;
+    int begin_of_window = 0;
+    for (int r0 = 0; r0 < tokens || r0 == 0; r0 += range) {  // most tables: one window of the bucket's tokens
+        const int rows = min(range, tokens - r0);
+        if (r0) {
+            for (int i = tid; i < kSortWarps * range; i += kSortThreads) cell[i] = 0;
+            __syncthreads();
         }
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            const uint32_t v = counted(t[k]);
-            const int of = v == kNone ? buckets : (int)(v & (buckets - 1));
-            below += of < bucket;
-            if (of == bucket) atomicAdd(mine + (v >> bits), 1);
-            if (__any_sync(0xffffffffu, of == bucket) && group < 64) seen |= 1ull << group;
-            group++;
+        const auto row_of = [&](uint2 entry) {  // of the window, -1 where it is of none
+            const int row = (int)entry.x - r0;
+            return entry.x != none.x && row >= 0 && row < rows ? row : -1;
+        };
+        int below = over([&](uint2 entry) {
+            const int row = row_of(entry);
+            const uint32_t in = __ballot_sync(0xffffffffu, row >= 0);
+            const int one = __shfl_sync(0xffffffffu, row, __ffs(in) - 1);
+            const uint32_t same = __ballot_sync(0xffffffffu, row == one);  // a frequent token fills whole groups
+            if (row >= 0 && (row != one || lane == __ffs(in) - 1)) atomicAdd(mine + row, row == one ? __popc(same) : 1);
+        });
+        if (r0 == 0) {  // what the tiles hold of the buckets before this one
+            below = __reduce_add_sync(0xffffffffu, below);
+            if (lane == 0) atomicAdd(&base, below);
         }
-    }
-    if (bad) flag(status, PCFGNAT_STATUS_BAD_INDEX);
-    below = __reduce_add_sync(0xffffffffu, below);
-    if (lane == 0) warp_below[warp] = below;
-    __syncthreads();
-    // where every token of the block begins, and within it every warp
-    int mine_total = 0;
-    if (tid < range)
-        for (int w = 0; w < kSortWarps; w++) mine_total += cell[w * range + tid];
-    int scan = mine_total;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, scan, o);
-        if (lane >= o) scan += x;
-    }
-    if (lane == 31) warp_sum[warp] = scan;
-    __syncthreads();
-    if (tid < range) {
-        int next = scan - mine_total;
-        for (int w = 0; w < kSortWarps; w++) next += warp_below[w] + (w < warp ? warp_sum[w] : 0);
+        __syncthreads();
+        if (r0 == 0) begin_of_window = base;
+        // where every token begins, and within it every warp
+        int sum = 0;
+        if (tid < rows)
 #pragma unroll 8
-        for (int w = 0; w < kSortWarps; w++) {
-            const int c = cell[w * range + tid];
-            cell[w * range + tid] = next;
-            next += c;
-        }
-        const int64_t v = ((int64_t)tid << bits) + bucket;
-        if (v < V) sorted.row_end[v] = next;
-        if (tid == range - 1 && bucket == buckets - 1) *sorted.total = next;
-    }
-    __syncthreads();
-    group = 0;
-    for (int i0 = first; i0 < last; i0 += 32 * kAhead, group += kAhead) {
-        const uint32_t some = group < 64 ? (uint32_t)(seen >> group) & ((1u << kAhead) - 1) : (1u << kAhead) - 1;
-        if (!some) continue;
-        uint32_t v[kAhead];
+            for (int w = 0; w < kSortWarps; w++) sum += cell[w * range + tid];
+        int scan = sum;
 #pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            const int i = i0 + k * 32 + lane;
-            v[k] = (some >> k & 1) && i < last ? counted(words[i]) : kNone;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += x;
         }
-#pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            // one token after the other, as few of them are the block's
-            uint32_t todo = __ballot_sync(0xffffffffu, v[k] != kNone && (int)(v[k] & (buckets - 1)) == bucket);
-            while (todo) {
-                const uint32_t one = __shfl_sync(0xffffffffu, v[k], __ffs(todo) - 1);
-                const uint32_t same = __ballot_sync(0xffffffffu, v[k] == one);
-                const int row = (int)(one >> bits), from = mine[row];
+        if (lane == 31) warp_sum[warp] = scan;
+        __syncthreads();
+        if (tid < rows) {
+            int next = begin_of_window + scan - sum;
+            for (int w = 0; w < warp; w++) next += warp_sum[w];
+#pragma unroll 8
+            for (int w = 0; w < kSortWarps; w++) {
+                const int c = cell[w * range + tid];
+                cell[w * range + tid] = next;
+                next += c;
+            }
+            sorted.row_end[((int64_t)(r0 + tid) << kBucketBits) + bucket] = next;
+        }
+        begin_of_window += __reduce_add_sync(0xffffffffu, warp_sum[lane]);
+        __syncthreads();
+        over([&](uint2 entry) {
+            const int row = row_of(entry);
+            for (uint32_t todo = __ballot_sync(0xffffffffu, row >= 0); todo;) {  // one token after the other
+                const int one = __shfl_sync(0xffffffffu, row, __ffs(todo) - 1);
+                const uint32_t same = __ballot_sync(0xffffffffu, row == one);
+                const int from = mine[one];
                 __syncwarp();
-                if (v[k] == one) {
+                if (lane == 0) mine[one] = from + __popc(same);
+                if (row == one) {
                     const int at = from + __popc(same & ((1u << lane) - 1));
-                    sorted.token[at] = (int)one, sorted.at[at] = i0 + k * 32 + lane;
+                    sorted.token[at] = ((one + r0) << kBucketBits) + bucket, sorted.at[at] = (int)entry.y;
                 }
-                if (lane == 0) mine[row] = from + __popc(same);
                 __syncwarp();
                 todo &= ~same;
             }
-        }
+        });
+        __syncthreads();
     }
+    if (bucket == kBuckets - 1 && tid == 0) *sorted.total = begin_of_window;
 }
 
 // A finished sum into the table.  Every number of the table gets at most one sum per call, so adding to a float32 table by a
@@ -232,20 +354,48 @@ struct Pieces {
     int length;    // entries of a warp, kSumWarps warps to a piece
 };
 
-// A block adds up a piece of the list for a tile of columns, a warp an equal share of it, a lane REP times VEC columns (32 * VEC
-// apart).  A warp's runs that cross its borders are joined in shared memory, in the list's order, and so are given on only where
-// they cross the piece's.
-template <typename G, typename W, int VEC, int REP>
+// Columns of a block: 512 bytes of a gradient's row.
+template <typename G>
+constexpr int kColumns = 512 / (int)sizeof(G);
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void *to, const void *from) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_address(to)), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(shared_address(to)), "l"(from) : "memory");
+}
+
+// A tile's columns of a gradient's row into shared memory, by a warp.  ALIGNED: in 16-byte vectors, all of them there.
+template <typename G, bool ALIGNED>
+__device__ __forceinline__ void stage_row(G *to, const G *from, int columns, int lane) {
+    if constexpr (ALIGNED) {
+        constexpr int kVec = 16 / sizeof(G);
+        if (lane * kVec < columns) copy_async<16>(to + lane * kVec, from + lane * kVec);
+    } else {
+#pragma unroll
+        for (int k = 0; k < kColumns<G> / 32; k++) {
+            const int c = k * 32 + lane;
+            if (c >= columns) continue;
+            if constexpr (sizeof(G) == 4) copy_async<4>(to + c, from + c);
+            else to[c] = from[c];
+        }
+    }
+}
+
+// A block adds up a piece of the list for a tile of columns, a warp an equal share of it: seven rows on their way to shared memory
+// while one is added.  A warp's runs that cross its borders are joined in shared memory, in the list's order, and so are given on only
+// where they cross the piece's.  A lane's columns lie side by side where rows of table and gradient allow vectors, else 32 apart.
+template <typename G, typename W, bool ALIGNED>
 __global__ void __launch_bounds__(32 * kSumWarps)
     embed_sum_kernel(const G *__restrict__ grad, int64_t g_stride, int H, Pieces p, W *dw, int64_t dw_stride, float scale,
                      int accumulate) {
-    using Raw = typename RawVec<VEC * sizeof(G)>::type;
-    constexpr int kTile = 32 * VEC * REP;
-    __shared__ float crossing[kSumWarps][2][kTile];
+    constexpr int kCols = kColumns<G>, kMine = kCols / 32;
+    __shared__ __align__(16) G staged[kSumWarps][kAhead][kCols];
+    __shared__ float crossing[kSumWarps][2][kCols];
     __shared__ int4 ends[kSumWarps];  // of a warp's share: first and last token, whether those runs go on before and behind it
     chain_begin();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tile = blockIdx.y * kTile, c = tile + lane * VEC;  // of the lane's columns, the first
+    const int tile = blockIdx.y * kCols, columns = H - tile;
     const int total = *p.sorted.total;
     const int64_t begin64 = ((int64_t)blockIdx.x * kSumWarps + warp) * p.length;
     const int *token = p.sorted.token;
@@ -253,63 +403,75 @@ __global__ void __launch_bounds__(32 * kSumWarps)
     if (begin64 < total) {
         const int begin = (int)begin64, end = min(begin + p.length, total);
         const int before = begin > 0 ? token[begin - 1] : -1, after = end < total ? token[end] : -1;
-        float acc[REP][VEC] = {};
-        int run = token[begin];
+        int my_token = begin + lane < end ? token[begin + lane] : -1, my_at = begin + lane < end ? p.sorted.at[begin + lane] : 0;
+        int run = __shfl_sync(0xffffffffu, my_token, 0);
         bool began_before = run == before;
-        if (lane == 0) {
-            const int tail = token[end - 1];
-            ends[warp] = make_int4(run, tail, run == before, tail == after);
+        if (lane == 0) ends[warp].x = run, ends[warp].z = run == before;
+#pragma unroll
+        for (int j = 0; j < kAhead; j++) {
+            const int at = __shfl_sync(0xffffffffu, my_at, j);
+            if (begin + j < end) stage_row<G, ALIGNED>(staged[warp][j], grad + at * g_stride + tile, columns, lane);
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        for (int i0 = begin; i0 < end; i0 += 32) {
-            const int count = min(32, end - i0);
-            const int my_token = lane < count ? token[i0 + lane] : -1, my_at = lane < count ? p.sorted.at[i0 + lane] : 0;
-            const int behind = i0 + count < end ? token[i0 + count] : -1;
-            for (int j0 = 0; j0 < count; j0 += kAhead) {
-                Raw raw[kAhead][REP];
+        float acc[kMine] = {};
+        int slot = 0;
+        int ahead_at = my_at;  // positions of the 32 entries that hold the one kAhead further on
+        int ahead_base = begin;
+#pragma unroll 1
+        for (int i = begin; i < end; i++) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+            __syncwarp();
+            const G *row = staged[warp][slot];
+            if constexpr (ALIGNED) {
+                float x[kMine];
+                unpack_vec<G, kMine>(*reinterpret_cast<const uint4 *>(row + kMine * lane), x);
 #pragma unroll
-                for (int j = 0; j < kAhead; j++) {
-                    const G *row = grad + __shfl_sync(0xffffffffu, my_at, (j0 + j) & 31) * g_stride;
+                for (int k = 0; k < kMine; k++) acc[k] += x[k];
+            } else {
 #pragma unroll
-                    for (int q = 0; q < REP; q++)
-                        if (j0 + j < count && c + q * 32 * VEC < H) raw[j][q] = __ldg(reinterpret_cast<const Raw *>(row + c + q * 32 * VEC));
-                }
+                for (int k = 0; k < kMine; k++) acc[k] += num_to_float<G>(row[k * 32 + lane]);
+            }
+            __syncwarp();  // the row has been read
+            const int ahead = i + kAhead;
+            if (ahead - ahead_base >= 32) {
+                ahead_base += 32;
+                ahead_at = ahead_base + lane < end ? p.sorted.at[ahead_base + lane] : 0;
+            }
+            const int at = __shfl_sync(0xffffffffu, ahead_at, ahead - ahead_base);
+            if (ahead < end) stage_row<G, ALIGNED>(staged[warp][slot], grad + at * g_stride + tile, columns, lane);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            slot = slot + 1 == kAhead ? 0 : slot + 1;
+            // the next entry's token
+            int next = -1;
+            if ((i + 1 - begin) % 32 == 0) my_token = i + 1 + lane < end ? token[i + 1 + lane] : -1;
+            next = __shfl_sync(0xffffffffu, my_token, (i + 1 - begin) & 31);
+            if (i + 1 == end) next = -1;
+            if (next == run) continue;
+            const bool goes_on = next < 0 && run == after;
+            if (began_before || goes_on) {
+                float *to = crossing[warp][began_before ? 0 : 1];
 #pragma unroll
-                for (int j = 0; j < kAhead; j++) {
-                    const int next_of = __shfl_sync(0xffffffffu, my_token, (j0 + j + 1) & 31);
-                    if (j0 + j >= count) continue;  // the same for the whole warp
+                for (int k = 0; k < kMine; k++) to[ALIGNED ? kMine * lane + k : k * 32 + lane] = acc[k];
+            } else if constexpr (ALIGNED) {
+                if (kMine * lane < columns) write_row<W, kMine>(dw + run * dw_stride + tile + kMine * lane, acc, scale, accumulate);
+            } else {
 #pragma unroll
-                    for (int q = 0; q < REP; q++) {
-                        float x[VEC];
-                        unpack_vec<G, VEC>(raw[j][q], x);
-#pragma unroll
-                        for (int k = 0; k < VEC; k++) acc[q][k] += x[k];
-                    }
-                    const int next = j0 + j + 1 == count ? behind : next_of;
-                    if (next == run) continue;
-                    const bool goes_on = next < 0 && run == after;
-#pragma unroll
-                    for (int q = 0; q < REP; q++) {
-                        if (began_before || goes_on) {
-                            float *to = crossing[warp][began_before ? 0 : 1] + q * 32 * VEC + lane * VEC;
-#pragma unroll
-                            for (int k = 0; k < VEC; k++) to[k] = acc[q][k];
-                        } else if (c + q * 32 * VEC < H) {
-                            write_row<W, VEC>(dw + run * dw_stride + c + q * 32 * VEC, acc[q], scale, accumulate);
-                        }
-#pragma unroll
-                        for (int k = 0; k < VEC; k++) acc[q][k] = 0.f;
-                    }
-                    run = next;
-                    began_before = false;
+                for (int k = 0; k < kMine; k++) {
+                    const float one[1] = {acc[k]};
+                    if (k * 32 + lane < columns) write_row<W, 1>(dw + run * dw_stride + tile + k * 32 + lane, one, scale, accumulate);
                 }
             }
+#pragma unroll
+            for (int k = 0; k < kMine; k++) acc[k] = 0.f;
+            if (next < 0 && lane == 0) ends[warp].y = run, ends[warp].w = run == after;
+            run = next;
+            began_before = false;
         }
     }
     __syncthreads();
     // a thread per column: what the warps left, in the list's order
-    for (int col = threadIdx.x; col < kTile; col += 32 * kSumWarps) {
-        const int cc = tile + col;
-        if (cc >= H) continue;
+    const int col = threadIdx.x, cc = tile + col;
+    if (col < kCols && cc < H) {
         float *give = p.parts + (int64_t)blockIdx.x * 2 * H + cc;
         float acc[1] = {0.f};
         bool from_outside = false, open = false;
@@ -380,23 +542,41 @@ int widest(uintptr_t bits, int size) {  // bytes of the widest vector that addre
     return size;
 }
 
-// Entries of a warp: eight loads of a lane in flight, more where that made over 2 048 pieces.
+// Entries of a warp: eight, more where that made over 2 048 pieces.
 int warp_entries(int64_t n) {
     const int64_t even = (n + 2048 * kSumWarps - 1) / (2048 * kSumWarps);
-    return (int)((even + kAhead - 1) / kAhead * kAhead) + (even == 0 ? kAhead : 0);
+    return (int)(even < kShare ? kShare : (even + kShare - 1) / kShare * kShare);
 }
 int64_t piece_count(int64_t n) {
     const int64_t length = (int64_t)warp_entries(n) * kSumWarps;
     return (n + length - 1) / length;
 }
 
-constexpr size_t round16(size_t x) { return (x + 15) / 16 * 16; }
+struct Scratch {
+    Sorted sorted;
+    float *parts;
+    size_t bytes;
+    Scratch(char *at, int64_t n, int64_t V, int H) {
+        bytes = 0;
+        const auto take = [&](size_t size) {
+            char *p = at + bytes;
+            bytes += (size + 15) / 16 * 16;
+            return p;
+        };
+        const size_t tiles = (size_t)((n + kTile - 1) / kTile);
+        sorted.total = reinterpret_cast<int *>(take(sizeof(int)));
+        sorted.token = reinterpret_cast<int *>(take((size_t)n * sizeof(int)));
+        sorted.at = reinterpret_cast<int *>(take((size_t)n * sizeof(int)));
+        sorted.row_end = reinterpret_cast<int *>(take((size_t)V * sizeof(int)));
+        sorted.grouped = reinterpret_cast<uint2 *>(take(tiles * kTile * sizeof(uint2)));
+        sorted.bucket_begin = reinterpret_cast<int *>(take(tiles * (kBuckets + 1) * sizeof(int)));
+        parts = reinterpret_cast<float *>(take((size_t)piece_count(n) * 2 * H * sizeof(float)));
+    }
+};
 
 }  // namespace
 
-size_t embed_workspace_bytes(int64_t n, int64_t V, int H) {
-    return 16 + 2 * round16((size_t)n * sizeof(int)) + round16((size_t)V * sizeof(int)) + (size_t)piece_count(n) * 2 * H * sizeof(float);
-}
+size_t embed_workspace_bytes(int64_t n, int64_t V, int H) { return Scratch(nullptr, n, V, H).bytes; }
 
 int launch_embed(const void *weight, int dtype, int64_t w_stride, int64_t V, int H, const int64_t *tokens, int64_t n, float scale,
                  void *out, int *status, cudaStream_t st) {
@@ -427,66 +607,59 @@ int launch_embed(const void *weight, int dtype, int64_t w_stride, int64_t V, int
 int launch_embed_backward(const void *grad, int dtype, int64_t g_stride, const int64_t *tokens, int64_t n, int64_t V, int H, float scale,
                           int has_padding, int64_t padding, void *dw, int dw_dtype, int64_t dw_stride, int accumulate, void *workspace,
                           int *status, cudaStream_t st) {
-    char *ws = static_cast<char *>(workspace);
-    const size_t list = round16((size_t)n * sizeof(int));
-    const Sorted sorted{reinterpret_cast<int *>(ws + 16), reinterpret_cast<int *>(ws + 16 + list),
-                        reinterpret_cast<int *>(ws + 16 + 2 * list), reinterpret_cast<int *>(ws)};
-    float *parts = reinterpret_cast<float *>(ws + 16 + 2 * list + round16((size_t)V * sizeof(int)));
-    const size_t dw_size = dw_dtype == PCFGNAT_DTYPE_F32 ? 4 : 2;
-    int bits = 7;  // 128 blocks: as many as one of 1 024 threads each per SM gives
-    while ((V + (1ll << bits) - 1) >> bits > kMaxRange) bits++;
-    const int range = (int)((V + (1ll << bits) - 1) >> bits);
+    const Scratch scratch(static_cast<char *>(workspace), n, V, H);
+    const Sorted &sorted = scratch.sorted;
+    const int64_t dw_size = dw_dtype == PCFGNAT_DTYPE_F32 ? 4 : 2;
+    const int tiles = (int)((n + kTile - 1) / kTile), zeroing = accumulate ? 0 : sm_count();
+    const int range = (int)std::min<int64_t>(kMaxRange, (V + kBuckets - 1) / kBuckets);
     const size_t smem = (size_t)kSortWarps * range * sizeof(int);
     cudaError_t e = ensure_dynamic_smem(embed_sort_kernel, smem);
     if (e != cudaSuccess) return PCFGNAT_ERR_CUDA;
+    // the table is set to zero beside the sorting, a third of it beside the first, shorter kernel
+    const int64_t third = n ? V / 3 : V;
+    const Zeroed first{static_cast<char *>(dw), 0, third, H * dw_size, dw_stride * dw_size};
+    const Zeroed rest{static_cast<char *>(dw), third, V, H * dw_size, dw_stride * dw_size};
     const uint32_t skip = has_padding && padding >= 0 && padding < V ? (uint32_t)padding : 0xffffffffu;
-    embed_sort_kernel<<<(1u << bits) + (accumulate ? 0u : (unsigned)sm_count()), kSortThreads, smem, st>>>(
-        tokens, (int)n, (int)V, skip, bits, range, sorted, static_cast<char *>(dw), (int)(H * dw_size), (int64_t)(dw_stride * dw_size),
-        status);
+    if (tiles + zeroing == 0) return PCFGNAT_OK;
+    embed_group_kernel<<<(unsigned)(tiles + zeroing), kTile, 0, st>>>(tokens, (int)n, (int)V, skip, tiles, sorted, first, status);
     e = cudaGetLastError();
     if (e != cudaSuccess || n == 0) return cuda_rc(e);
-    const Pieces p{sorted, parts, warp_entries(n)};
+    // every further kernel waits for the one before it to end, but may be scheduled before that
+    const auto launch = [&](auto kernel, dim3 grid, unsigned threads, size_t bytes, auto... args) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = grid;
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = bytes;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, kernel, args...);
+    };
+    e = launch(embed_sort_kernel, dim3(kBuckets + zeroing), kSortThreads, smem, (int)V, tiles, range, sorted, rest);
+    if (e != cudaSuccess) return PCFGNAT_ERR_CUDA;
+    const Pieces p{sorted, scratch.parts, warp_entries(n)};
     const unsigned pieces = (unsigned)piece_count(n);
     return with_dtype(dtype, [&](auto g) {
         using G = decltype(g);
         const auto run = [&](auto w) {
             using W = decltype(w);
-            // a lane's columns: as many of the gradient's as 16 bytes hold, where both rows' addresses allow whole vectors
             const auto bits = [&](const void *a, int64_t stride, size_t size) {
                 return reinterpret_cast<uintptr_t>(a) | (uintptr_t)(stride * size) | (uintptr_t)(H * size);
             };
-            const int wide_g = widest(bits(grad, g_stride, sizeof(G)), sizeof(G)) / (int)sizeof(G);
-            const int wide_w = widest(bits(dw, dw_stride, sizeof(W)), sizeof(W)) / (int)sizeof(W);
-            // every kernel waits for the one before it to end, but may be scheduled before that
-            const auto launch = [&](auto kernel, unsigned tiles, unsigned threads, auto... args) {
-                cudaLaunchConfig_t cfg = {};
-                cfg.gridDim = dim3(pieces, tiles);
-                cfg.blockDim = dim3(threads);
-                cfg.stream = st;
-                cudaLaunchAttribute attr[1];
-                attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-                attr[0].val.programmaticStreamSerializationAllowed = 1;
-                cfg.attrs = attr;
-                cfg.numAttrs = 1;
-                return cudaLaunchKernelEx(&cfg, kernel, args...);
+            const bool aligned = widest(bits(grad, g_stride, sizeof(G)), sizeof(G)) == 16 && widest(bits(dw, dw_stride, sizeof(W)), sizeof(W)) == 16;
+            const dim3 grid(pieces, (unsigned)((H + kColumns<G> - 1) / kColumns<G>));
+            const auto sum = [&](auto kernel) {
+                return launch(kernel, grid, 32 * kSumWarps, 0, static_cast<const G *>(grad), g_stride, H, p, static_cast<W *>(dw),
+                              dw_stride, scale, accumulate);
             };
-            const auto sum = [&](auto vec, auto rep) {
-                constexpr int VEC = decltype(vec)::value, REP = decltype(rep)::value;
-                return launch(embed_sum_kernel<G, W, VEC, REP>, (unsigned)((H + 32 * VEC * REP - 1) / (32 * VEC * REP)), 32 * kSumWarps,
-                              static_cast<const G *>(grad), g_stride, H, p, static_cast<W *>(dw), dw_stride, scale, accumulate);
-            };
-            constexpr int kWide = 16 / sizeof(G), kWideW = 16 / sizeof(W) < kWide ? 16 / sizeof(W) : kWide;
-            using std::integral_constant;
-            cudaError_t rc;
-            if (wide_g >= kWide && wide_w >= kWideW && H % kWide == 0) rc = sum(integral_constant<int, kWide>(), integral_constant<int, 1>());
-            else if (wide_g >= 2 && wide_w >= 2) rc = sum(integral_constant<int, 2>(), integral_constant<int, 2>());
-            else rc = sum(integral_constant<int, 1>(), integral_constant<int, 4>());
-            if (rc != cudaSuccess) return (int)PCFGNAT_ERR_CUDA;
-            if (pieces > 1)  // one piece has no border
-                rc = launch(embed_join_kernel<W>, (unsigned)((H + kJoinColumns - 1) / kJoinColumns), 32 * kJoinGroups, H, p,
+            cudaError_t rc = aligned ? sum(embed_sum_kernel<G, W, true>) : sum(embed_sum_kernel<G, W, false>);
+            if (rc == cudaSuccess && pieces > 1)  // one piece has no border
+                rc = launch(embed_join_kernel<W>, dim3(pieces, (unsigned)((H + kJoinColumns - 1) / kJoinColumns)), 32 * kJoinGroups, 0, H, p,
                             static_cast<W *>(dw), dw_stride, scale, accumulate);
-            if (rc != cudaSuccess) return (int)PCFGNAT_ERR_CUDA;
-            return cuda_rc(cudaGetLastError());
+            return rc == cudaSuccess ? (int)PCFGNAT_OK : (int)PCFGNAT_ERR_CUDA;
         };
         if (dw_dtype == PCFGNAT_DTYPE_F32) return run(float());
         if (dw_dtype == dtype) return run(g);

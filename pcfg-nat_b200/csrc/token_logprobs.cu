@@ -97,10 +97,8 @@ __device__ __forceinline__ uint32_t rank_bits(float x) {
 __device__ __forceinline__ uint64_t entry_key(float x, int index) {
     return (uint64_t)rank_bits(x) << 32 | (uint32_t)~index;
 }
-__device__ __forceinline__ float key_value(uint64_t k) {
-    const uint32_t b = (uint32_t)(k >> 32);
-    return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
-}
+__device__ __forceinline__ float rank_value(uint32_t b) { return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b); }
+__device__ __forceinline__ float key_value(uint64_t k) { return rank_value((uint32_t)(k >> 32)); }
 __device__ __forceinline__ int key_index(uint64_t k) { return (int)~(uint32_t)k; }
 
 struct Rows {
@@ -188,8 +186,9 @@ __device__ __forceinline__ void best_entries(Team<NT> &t, const Part<T> &p, int 
     constexpr int kVec = RowCut<T>::kVec, kWarps = Team<NT>::kWarps;
     const int warp = tid >> 5, lane = tid & 31;
     const uint32_t least = t.bound;
+    const float at_least = least ? rank_value(least) : neg_inf();
     const auto offer = [&](float x, int index) {
-        if (x == neg_inf() || rank_bits(x) < least) return;
+        if (x == neg_inf() || !(x >= at_least)) return;
         const int at = atomicAdd(&t.n_found, 1);
         if (at < Team<NT>::kCandidates) t.found[at] = entry_key(x, index);
     };
@@ -209,6 +208,8 @@ __device__ __forceinline__ void best_entries(Team<NT> &t, const Part<T> &p, int 
 #pragma unroll
         for (int k = 0; k < kUnroll; k++) {
             if (at[k] >= p.last) continue;
+            const uint32_t word[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+            if (!(max_of_words<T, 4>(word) >= at_least)) continue;  // as in most vectors
             float x[kVec];
             unpack_vec<T, kVec>(raw[k], x);
 #pragma unroll

@@ -26,6 +26,16 @@ from . import pcfg_loss as _ops
 MAX_TOP = 32  # PCFGNAT_MAX_TOP
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # PCFGNAT_DTYPE_*
 
+def _first_derivative(backward):
+    """``once_differentiable``, whose guard is only set up where a graph of the backward pass is asked for."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
 TokenLogprobs = namedtuple("TokenLogprobs", "logprob entropy top_logprob top_index")
 
 
@@ -160,7 +170,7 @@ class TokenLogprobsFunc(Function):
         return logprob, ent, top_lp, top_ix
 
     @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, g_logprob, g_entropy, g_top, _):
         logits, tokens, kept, ent, top_ix = ctx.saved_tensors
         if not ctx.needs_input_grad[0] or (g_logprob is None and g_entropy is None and g_top is None):
@@ -262,7 +272,7 @@ class EmbedTokensFunc(Function):
         return _embed(weight, tokens, scale)
 
     @staticmethod
-    @once_differentiable
+    @_first_derivative
     def backward(ctx, grad_out):
         if not ctx.needs_input_grad[0]:
             return None, None, None, None
@@ -338,40 +348,44 @@ def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
     outs = grads if out is None else listed(out)
     if len(outs) != len(grads):
         raise RuntimeError("out must hold one tensor per gradient")
-    if any(g is None for g in grads):
-        there = [i for i, g in enumerate(grads) if g is not None]
-        grads, outs = [grads[i] for i in there], [outs[i] for i in there]
-        outs = grads if out is None else outs
-    if not grads:
-        return torch.zeros((), dtype=torch.float32, device=torch.device("cuda", torch.cuda.current_device()))
     # one plain pass over the list for each question: a model has hundreds of gradients, and the kernels are done with them sooner
-    every = grads if outs is grads else grads + outs
+    every = grads if out is None else grads + outs
     try:
-        at, size = list(map(torch.Tensor.data_ptr, every)), list(map(torch.Tensor.numel, every))
-        index = set(map(torch.Tensor.get_device, every))
+        at = list(map(torch.Tensor.data_ptr, every))
     except TypeError:
-        raise RuntimeError("gradients and outputs must be tensors") from None
+        if any(g is not None and not isinstance(g, torch.Tensor) for g in every):
+            raise RuntimeError("gradients and outputs must be tensors") from None
+        there = [i for i, g in enumerate(grads) if g is not None]
+        grads = [grads[i] for i in there]
+        return clip_grad_norm_(grads, max_norm, None if out is None else [outs[i] for i in there], grad_scale)
     n = len(grads)
+    if n == 0:
+        return torch.zeros((), dtype=torch.float32, device=torch.device("cuda", torch.cuda.current_device()))
+    size = list(map(torch.Tensor.numel, every))
+    index = set(map(torch.Tensor.get_device, every))
     if len(index) != 1 or min(index) < 0:
         raise RuntimeError("the gradients and outputs must be CUDA tensors on one device")
-    kind = [_DTYPES.get(t.dtype) for t in every]
-    if None in kind:
+    kind = [t.dtype for t in every]
+    if not _DTYPES.keys() >= set(kind):
         raise RuntimeError("gradients and outputs must be float32, float16 or bfloat16")
+    kind = [_DTYPES[t] for t in kind] if len(set(kind)) > 1 else [_DTYPES[kind[0]]] * len(kind)
     if not all(map(torch.Tensor.is_contiguous, every)):
         for g, o in zip(grads, outs):
             if not _dense(g):
                 raise RuntimeError("a gradient must be dense: call contiguous() first")
             if o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
                 raise RuntimeError("an output must have its gradient's layout")
-    if outs is not grads:
+    host = lambda code, v: array.array(code, v)  # read before the call returns
+    src, src_kind, numel = host("Q", at[:n]), host("i", kind[:n]), host("q", size[:n])
+    dst, dst_kind = src, src_kind
+    if out is not None:
         if size[:n] != size[n:]:
             raise RuntimeError("an output must have its gradient's shape")
         if any(k and k != j for j, k in zip(kind[:n], kind[n:])):
             raise RuntimeError("an output must be of its gradient's type or float32")
+        dst, dst_kind = host("Q", at[n:]), host("i", kind[n:])
     dev = grads[0].device
     lib = _cabi.lib()
-    host = lambda code, v: array.array(code, v)  # read before the call returns
-    src, dst, src_kind, dst_kind, numel = host("Q", at[:n]), host("Q", at[-n:]), host("i", kind[:n]), host("i", kind[-n:]), host("q", size[:n])
     head = lambda a: a.buffer_info()[0]
     with _on(dev):
         nbytes = lib.pcfgnat_clip_grad_norm_workspace_bytes(n)
