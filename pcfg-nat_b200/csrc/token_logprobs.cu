@@ -107,7 +107,10 @@ struct Rows {
     int V;
     template <typename T>
     __device__ __forceinline__ const T *at(int64_t r) const {
-        return static_cast<const T *>(logits) + (r / inner) * stride_outer + (r % inner) * stride_inner;
+        const T *p = static_cast<const T *>(logits);
+        if (r < inner) return p + r * stride_inner;  // all rows at one stride: no division
+        const uint32_t outer = (uint32_t)r / (uint32_t)inner, rest = (uint32_t)r - outer * (uint32_t)inner;
+        return p + outer * stride_outer + rest * stride_inner;
     }
 };
 
@@ -133,6 +136,24 @@ struct Part {
     int head, first, last;  // vectors [first, last)
     int loose, vecs;        // numbers in no vector that this part takes, vectors of the whole row
     __device__ __forceinline__ int loose_at(int i) const { return i < head ? i : i + vecs * RowCut<T>::kVec; }
+    __device__ __forceinline__ Part(const Rows &rows, int64_t r, int rank, int parts) {
+        row = rows.at<T>(r);
+        const RowCut<T> cut(row, rows.V);
+        head = cut.head, vecs = cut.vecs;
+        vec = reinterpret_cast<const uint4 *>(row + cut.head);
+        const int share = (cut.vecs + parts - 1) / parts;
+        first = min(rank * share, cut.vecs), last = min(first + share, cut.vecs);
+        loose = rank == 0 ? cut.loose(rows.V) : 0;
+    }
+    // kUnroll vectors from number i on, NT apart; nothing but -inf behind the last.
+    template <int NT>
+    __device__ __forceinline__ void load(uint4 (&raw)[kUnroll], int i) const {
+#pragma unroll
+        for (int k = 0; k < kUnroll; k++) {
+            const uint32_t none = neg_inf_word<T>();
+            raw[k] = i + k * NT < last ? __ldg(vec + i + k * NT) : make_uint4(none, none, none, none);
+        }
+    }
 };
 
 // What a team of NT threads shares.
@@ -192,6 +213,14 @@ __device__ __forceinline__ void best_entries(Team<NT> &t, const Part<T> &p, int 
         const int at = atomicAdd(&t.n_found, 1);
         if (at < Team<NT>::kCandidates) t.found[at] = entry_key(x, index);
     };
+    const auto offer_vector = [&](const uint4 &raw, int i) {
+        const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+        if (!(max_of_words<T, 4>(word) >= at_least)) return;  // as in most vectors
+        float x[kVec];
+        unpack_vec<T, kVec>(raw, x);
+#pragma unroll
+        for (int j = 0; j < kVec; j++) offer(x[j], p.head + i * kVec + j);
+    };
     if (own_max != 0 && own_max >= least) t.again[atomicAdd(&t.n_again, 1)] = (uint16_t)tid;
     team_sync<NT>();
     // thread by thread of those, vector by vector, dealt out to all threads of the team
@@ -206,15 +235,8 @@ __device__ __forceinline__ void best_entries(Team<NT> &t, const Part<T> &p, int 
             if (at[k] < p.last) raw[k] = __ldg(p.vec + at[k]);
         }
 #pragma unroll
-        for (int k = 0; k < kUnroll; k++) {
-            if (at[k] >= p.last) continue;
-            const uint32_t word[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-            if (!(max_of_words<T, 4>(word) >= at_least)) continue;  // as in most vectors
-            float x[kVec];
-            unpack_vec<T, kVec>(raw[k], x);
-#pragma unroll
-            for (int j = 0; j < kVec; j++) offer(x[j], p.head + at[k] * kVec + j);
-        }
+        for (int k = 0; k < kUnroll; k++)
+            if (at[k] < p.last) offer_vector(raw[k], at[k]);
     }
     for (int i = tid; i < p.loose; i += NT) offer(num_to_float<T>(p.row[p.loose_at(i)]), p.loose_at(i));
     team_sync<NT>();
@@ -257,9 +279,64 @@ __device__ __forceinline__ void best_entries(Team<NT> &t, const Part<T> &p, int 
     }
 }
 
+__device__ __forceinline__ void leave_out(const Results &out, int64_t r, int tid) {
+    if (tid == 0) {
+        out.logprob[r] = 0.f;
+        if (out.entropy) out.entropy[r] = 0.f;
+        if (out.kept) out.kept[2 * r] = out.kept[2 * r + 1] = 0.f;
+    }
+    if (tid < out.top) out.top_logprob[r * out.top + tid] = 0.f, out.top_index[r * out.top + tid] = -1;
+}
+
+// The end of a row, by one warp: `a` is the whole row's, x its number at the given token.
+template <int NT, bool ENTROPY>
+__device__ __forceinline__ void write_out(const Results &out, const Team<NT> &t, const Stats &a, int64_t r, bool inside, float x,
+                                          int lane) {
+    const float log_s = logf(a.s);  // -inf for a row of nothing but -inf
+    const int top = out.top;
+    if (lane == 0) {
+        if (!inside) flag(out.status, PCFGNAT_STATUS_BAD_INDEX);
+        out.logprob[r] = !inside ? CUDART_NAN_F : a.s == 0.f ? neg_inf() : (x - a.m) - log_s;
+        if (ENTROPY) out.entropy[r] = a.s == 0.f ? 0.f : log_s - kLn2 * (a.u / a.s);
+        if (out.kept) out.kept[2 * r] = a.m, out.kept[2 * r + 1] = log_s;
+    }
+    if (lane < top) {
+        const uint64_t key = a.s > 0.f ? t.best[lane] : 0;
+        // a row that is no distribution is NaN; an alternative that does not exist has no probability
+        out.top_logprob[r * top + lane] = key ? (key_value(key) - a.m) - log_s : a.s >= 0.f ? neg_inf() : CUDART_NAN_F;
+        out.top_index[r * top + lane] = key ? key_index(key) : -1;
+    }
+}
+
+// What every thread found of its part: the whole part's in warp 0, and what the search for alternatives starts from.
+template <int NT>
+__device__ __forceinline__ Stats join_team(Team<NT> &t, Stats a, uint32_t own_max, int top, int tid) {
+    const int warp = tid >> 5, lane = tid & 31;
+    if (top) t.maxima[tid] = own_max;
+    a = join_lanes(a);
+    if (Team<NT>::kWarps > 1 && lane == 0) t.part[warp] = a;
+    team_sync<NT>();
+    if (warp == 0) {
+        if (Team<NT>::kWarps > 1) a = join_lanes(lane < Team<NT>::kWarps ? t.part[lane] : Stats());
+        if (top) {
+            const uint32_t least = a.s > 0.f ? lower_bound_of_top<NT>(t, top, lane) : 0xffffffffu;  // that many or none
+            if (lane == 0) t.bound = least, t.n_found = t.n_again = 0;
+            t.best[lane] = 0;
+        }
+    }
+    return a;
+}
+// 0: no entry but -inf (or NaN, where nothing is chosen)
+__device__ __forceinline__ uint32_t maximum_of(const Stats &a) { return a.s > 0.f ? rank_bits(a.m) : 0u; }
+
+// Blocks that fit an SM.  More hide more of the memory's latency until their registers run out: with 40 000 numbers a row,
+// float32 rows 61, 51 and 56 us with 9, 10 and 12 blocks, halves 57, 57 and 60 us for 2 272 rows with eight alternatives.
+template <typename T, int NT>
+constexpr int kResident = NT == 512 ? 2 : NT == 32 || sizeof(T) == 4 ? 10 : 9;
+
 // A team of NT threads per row or, in a cluster, per part of a row; the first block of a cluster joins the parts.
 template <typename T, int NT, bool ENTROPY>
-__global__ void __launch_bounds__(NT < 128 ? 128 : NT)
+__global__ void __launch_bounds__(NT < 128 ? 128 : NT, kResident<T, NT>)
     token_logprobs_kernel(Rows rows, int64_t n_rows, Given given, Results out) {
     constexpr int kTeams = NT < 128 ? 128 / NT : 1;
     __shared__ Team<NT> teams[kTeams];
@@ -269,54 +346,24 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT)
     const int parts = kTeams == 1 ? (int)cluster.num_blocks() : 1, rank = kTeams == 1 ? (int)cluster.block_rank() : 0;
     const int64_t r = kTeams == 1 ? (int64_t)(blockIdx.x / (unsigned)parts) : (int64_t)blockIdx.x * kTeams + threadIdx.x / NT;
     if (r >= n_rows) return;
-    const int V = rows.V, top = out.top;
+    const int top = out.top;
     const int64_t token = given.tokens[r];
     if (given.has_ignore && token == given.ignore) {
-        if (rank) return;
-        if (tid == 0) {
-            out.logprob[r] = 0.f;
-            if (out.entropy) out.entropy[r] = 0.f;
-            if (out.kept) out.kept[2 * r] = out.kept[2 * r + 1] = 0.f;
-        }
-        if (tid < top) out.top_logprob[r * top + tid] = 0.f, out.top_index[r * top + tid] = -1;
+        if (rank == 0) leave_out(out, r, tid);
         return;
     }
-    Part<T> p;
-    {
-        p.row = rows.at<T>(r);
-        const RowCut<T> cut(p.row, V);
-        p.head = cut.head, p.vecs = cut.vecs;
-        p.vec = reinterpret_cast<const uint4 *>(p.row + cut.head);
-        const int share = (cut.vecs + parts - 1) / parts;
-        p.first = min(rank * share, cut.vecs), p.last = min(p.first + share, cut.vecs);
-        p.loose = rank == 0 ? cut.loose(V) : 0;
-    }
+    const Part<T> p(rows, r, rank, parts);
+    const bool inside = token >= 0 && token < rows.V;
+    const float x_token = tid == 0 && inside ? num_to_float<T>(p.row[token]) : 0.f;  // needed at the end, on its way from here on
     Stats a;
     for (int i = p.first + tid; i < p.last; i += kUnroll * NT) {
         uint4 raw[kUnroll];
-#pragma unroll
-        for (int k = 0; k < kUnroll; k++) {
-            const uint32_t none = neg_inf_word<T>();
-            raw[k] = i + k * NT < p.last ? __ldg(p.vec + i + k * NT) : make_uint4(none, none, none, none);
-        }
+        p.template load<NT>(raw, i);
         take<T, ENTROPY>(a, raw);
     }
     if (tid < p.loose) take_one<ENTROPY>(a, num_to_float<T>(p.row[p.loose_at(tid)]));
-    const uint32_t own_max = a.s > 0.f ? rank_bits(a.m) : 0u;  // 0: no entry but -inf (or NaN, where nothing is chosen)
-    if (top) t.maxima[tid] = own_max;
-    a = join_lanes(a);
-    if (Team<NT>::kWarps > 1 && lane == 0) t.part[warp] = a;
-    team_sync<NT>();
-    if (warp == 0) {  // the rest is this warp's, but for the alternatives
-        if (Team<NT>::kWarps > 1) a = join_lanes(lane < Team<NT>::kWarps ? t.part[lane] : Stats());
-        if (top) {
-            const uint32_t least = a.s > 0.f ? lower_bound_of_top<NT>(t, top, lane) : 0xffffffffu;  // that many or none
-            if (lane == 0) t.bound = least, t.n_found = t.n_again = 0;
-            t.best[lane] = 0;
-        }
-    } else if (!top && parts == 1) {
-        return;
-    }
+    const uint32_t own_max = maximum_of(a);
+    a = join_team<NT>(t, a, own_max, top, tid);
     if (top) {
         team_sync<NT>();
         best_entries<T, NT>(t, p, top, own_max, tid);
@@ -345,26 +392,7 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT)
             __syncthreads();
         }
     }
-    if (warp) return;
-    const float log_s = logf(a.s);  // -inf for a row of nothing but -inf
-    if (lane == 0) {
-        float lp;
-        if (token < 0 || token >= V) {
-            lp = CUDART_NAN_F;
-            flag(out.status, PCFGNAT_STATUS_BAD_INDEX);
-        } else {
-            lp = a.s == 0.f ? neg_inf() : (num_to_float<T>(p.row[token]) - a.m) - log_s;
-        }
-        out.logprob[r] = lp;
-        if (ENTROPY) out.entropy[r] = a.s == 0.f ? 0.f : log_s - kLn2 * (a.u / a.s);
-        if (out.kept) out.kept[2 * r] = a.m, out.kept[2 * r + 1] = log_s;
-    }
-    if (lane < top) {
-        const uint64_t key = a.s > 0.f ? t.best[lane] : 0;
-        // a row that is no distribution is NaN; an alternative that does not exist has no probability
-        out.top_logprob[r * top + lane] = key ? (key_value(key) - a.m) - log_s : a.s >= 0.f ? neg_inf() : CUDART_NAN_F;
-        out.top_index[r * top + lane] = key ? key_index(key) : -1;
-    }
+    if (warp == 0) write_out<NT, ENTROPY>(out, t, a, r, inside, x_token, lane);
 }
 
 constexpr int kThreads = 256;
@@ -497,7 +525,6 @@ int launch_token_logprobs(const void *logits, int dtype, int64_t n, int64_t inne
         if (vecs <= 256) return run(std::integral_constant<int, 32>(), 1);
         int parts = 1;
         while (parts < 8 && n * parts * 2 <= 8 * sms && vecs >= (int64_t)parts * 2 * 256) parts *= 2;
-        if (n * parts > INT32_MAX) return (int)PCFGNAT_ERR_TOO_LARGE;
         if (parts == 8 && n * parts <= sms && vecs >= 8 * 1024) return run(std::integral_constant<int, 512>(), parts);
         return run(std::integral_constant<int, 128>(), parts);
     });

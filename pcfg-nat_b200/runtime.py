@@ -27,6 +27,7 @@ import torch
 
 from . import sharding
 from .custom_ops import pcfg_loss as ops
+from .custom_ops import vocabulary
 
 
 class _GraphedStep:
@@ -438,12 +439,21 @@ class GlanceStep(LossStep):
     Inputs (``load`` order): those of ``LossStep`` and prev_output_tokens [B,L] int64.  ``run()`` returns
     (tree [B,L] i64, sentence log-likelihood [B], arg-max tokens [B,L] i64, sampler outputs: the dict of
     ``glance_select`` — match mask, oracle tokens, kept positions, decoder input of the second pass).  The
-    sampler's normal draws are made inside the step into ``self.noise``."""
+    sampler's normal draws are made inside the step into ``self.noise``.
+
+    ``embedding``: the decoder's embedding table [V, H'] (the projection's ``weight`` itself where they are shared; read at every
+    run).  The sampler outputs then hold ``glat_embedded`` [B,L,H'] = ``embed_scale`` * embedding[decoder input] as well, what the
+    second pass begins with before positions are added."""
     kernels_per_step = 6  # proj_prepare, proj, proj_merge, loss_fwd, best_tree, glance_select
 
     def __init__(self, weight, B, L, T, device, use_graph=True, context_p=0.5, copy_chunks=2,
-                 strategy="number-random"):
+                 strategy="number-random", embedding=None, embed_scale=1.0):
         super().__init__(weight, B, L, T, device, use_graph, copy_chunks)
+        if embedding is not None and (embedding.dim() != 2 or embedding.device != self.weight.device):
+            raise RuntimeError("embedding must be a matrix [V, H] on the step's device")
+        self.embedding, self.embed_scale = embedding, float(embed_scale)
+        if embedding is not None:
+            self.kernels_per_step = 7  # and embed_rows
         self.context_p = float(context_p)
         self.strategy = strategy  # the criterion's --glance-strategy: "number-random", "cmlm" or None
         self.prev_output_tokens = torch.ones((B, L), dtype=torch.int64, device=self.device)
@@ -471,6 +481,9 @@ class GlanceStep(LossStep):
             self.uniform.uniform_()
         glance = k.glance_select(tree, em["argmax"], self.targets, self.prev_output_tokens, self.target_length,
                                  self.noise, self.context_p, self.strategy, self.uniform)
+        if self.embedding is not None:
+            glance["glat_embedded"] = vocabulary.embed_tokens(self.embedding.detach(), glance["glat_prev_output_tokens"],
+                                                              self.embed_scale)
         return tree, S[:, 0, 0], em["argmax"], glance
 
 

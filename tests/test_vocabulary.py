@@ -640,6 +640,40 @@ def test_the_shared_tables_gradient_from_both_ends(voc, ops):
 
 
 @gpu
+def test_the_glancing_step_embeds_the_second_passs_input(pkg, voc, ops, syn):
+    """GlanceStep(embedding=...) against the operators one by one, over a new batch in the same graph, and the shared table's
+    gradient from LossStep(proj_backward=True) completed by the embedding's."""
+    runtime = importlib.import_module("pcfg_nat_b200.runtime")
+    w = syn.Workload("ge", batch=4, vocab=2000, hidden=64, src_min=6, src_max=20, kind="glance")
+    b = syn.make_batch(w, seed=5)
+    weight = b.weight.cuda()
+    prev = torch.where(torch.arange(b.L)[None, :] < b.output_length[:, None], 3, 1)
+    batch = [b.hidden, b.links, b.output_length, b.targets, b.target_length, prev]
+    gs = runtime.GlanceStep(weight, b.B, b.L, b.T, "cuda:0", embedding=weight, embed_scale=8.0)
+    assert gs.kernels_per_step == runtime.GlanceStep.kernels_per_step + 1
+    for tensors in (batch, [t.flip(0) for t in batch]):
+        gs.load(*tensors)
+        glance = gs.run()[3]
+        tokens = glance["glat_prev_output_tokens"]
+        assert torch.equal(glance["glat_embedded"], (weight[tokens].float() * 8).half())
+        assert torch.equal(glance["glat_embedded"], voc.embed_tokens(weight, tokens, 8.0))
+    plain = runtime.GlanceStep(weight, b.B, b.L, b.T, "cuda:0", use_graph=False)
+    plain.load(*batch)
+    assert "glat_embedded" not in plain.run()[3]
+    with pytest.raises(RuntimeError, match="embedding must be"):
+        runtime.GlanceStep(weight, b.B, b.L, b.T, "cuda:0", embedding=weight.cpu())
+    ls = runtime.LossStep(weight, b.B, b.L, b.T, "cuda:0", proj_backward=True)
+    ls.load(*batch[:5])
+    d_weight = ls.run()[-1]
+    start = d_weight.clone()
+    g = torch.randn(tokens.shape + (64,), device="cuda").to(d_weight.dtype)
+    voc.embed_tokens_backward(g, tokens, d_weight, scale=8.0, padding_idx=1)
+    want, room = _grad64(g, tokens, 2000, 8.0, 1)
+    want = want + start.double()
+    _close(d_weight, want, room + U * want.abs(), d_weight.dtype)
+
+
+@gpu
 def test_on_another_stream_and_while_calls_overlap(voc):
     x, t = _random_logits((64, 20000), torch.bfloat16)
     w = torch.randn((20000, 128), device="cuda").bfloat16()
