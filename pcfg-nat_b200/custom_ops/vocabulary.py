@@ -162,7 +162,7 @@ class TokenLogprobsFunc(Function):
     @staticmethod
     def forward(ctx, logits, tokens, top, entropy, ignore):
         logprob, ent, top_lp, top_ix, kept = _token_logprobs(logits, tokens, top, entropy, ignore, True)
-        ctx.save_for_backward(logits, tokens, kept, ent, top_ix)
+        ctx.save_for_backward(logits, tokens.contiguous(), kept, ent, top_ix)
         ctx.top, ctx.ignore = top, ignore
         ctx.set_materialize_grads(False)
         if top_ix is not None:
@@ -172,12 +172,11 @@ class TokenLogprobsFunc(Function):
     @staticmethod
     @_first_derivative
     def backward(ctx, g_logprob, g_entropy, g_top, _):
-        logits, tokens, kept, ent, top_ix = ctx.saved_tensors
-        if not ctx.needs_input_grad[0] or (g_logprob is None and g_entropy is None and g_top is None):
+        if g_logprob is None and g_entropy is None and g_top is None:
             return None, None, None, None, None
+        logits, tokens, kept, ent, top_ix = ctx.saved_tensors
         V, dev = logits.shape[-1], logits.device
         inner, stride_outer, stride_inner = _logits_rows(logits)
-        tokens = tokens.contiguous()
         n = tokens.numel()
         # rows as far apart as the logits' own where those are padded: both then start at the same place of a 16-byte vector
         pitch = stride_inner if V <= stride_inner < V + 64 else V
@@ -244,22 +243,23 @@ def _embed(weight, tokens, scale):
     return out
 
 
-def _embed_backward(grad_out, tokens, d_weight, scale, padding, accumulate):
-    dt, dev = _numbers(grad_out, "grad_out"), grad_out.device
+def _embed_backward(g, tokens, d_weight, scale, padding, accumulate):  # on the tensors' device
+    dev = g.device
     V, H = d_weight.shape
     n = tokens.numel()
-    g = grad_out
-    rows = _rows(g) if H == 1 or g.stride(-1) == 1 else None
-    if rows is None or rows[0] != n and n > 1 or n > 1 and rows[2] < 0:  # not rows at one stride
-        g = g.contiguous()
-        rows = (n, 0, H)
+    stride = H
+    if not g.is_contiguous():
+        rows = _rows(g) if H == 1 or g.stride(-1) == 1 else None
+        if rows is None or rows[0] != n and n > 1:  # not rows at one stride
+            g = g.contiguous()
+        else:
+            stride = rows[2]
     lib = _cabi.lib()
     nbytes = lib.pcfgnat_embed_backward_workspace_bytes(n, V, H)
-    with _on(dev):
-        ws = tokens.new_empty(nbytes, dtype=torch.uint8)
-        rc = lib.pcfgnat_embed_backward(g.data_ptr(), dt, rows[2], tokens.data_ptr(), n, V, H, scale, *padding, d_weight.data_ptr(),
-                                        _DTYPES[d_weight.dtype], max(d_weight.stride(0), H), int(accumulate), ws.data_ptr(), nbytes,
-                                        _status_of(dev), _stream(dev))
+    ws = tokens.new_empty(nbytes, dtype=torch.uint8)
+    rc = lib.pcfgnat_embed_backward(g.data_ptr(), _DTYPES[g.dtype], stride, tokens.data_ptr(), n, V, H, scale, *padding, d_weight.data_ptr(),
+                                    _DTYPES[d_weight.dtype], max(d_weight.stride(0), H), int(accumulate), ws.data_ptr(), nbytes,
+                                    _status_of(dev), _stream(dev))
     _cabi.check(rc, "pcfgnat_embed_backward")
     return d_weight
 
@@ -267,19 +267,18 @@ def _embed_backward(grad_out, tokens, d_weight, scale, padding, accumulate):
 class EmbedTokensFunc(Function):
     @staticmethod
     def forward(ctx, weight, tokens, scale, padding):
-        ctx.save_for_backward(tokens)
+        out = _embed(weight, tokens, scale)  # checks them
+        ctx.save_for_backward(tokens.contiguous())
         ctx.scale, ctx.padding, ctx.table = scale, padding, weight.shape
-        return _embed(weight, tokens, scale)
+        return out
 
     @staticmethod
     @_first_derivative
     def backward(ctx, grad_out):
-        if not ctx.needs_input_grad[0]:
-            return None, None, None, None
         (tokens,) = ctx.saved_tensors
         with _on(grad_out.device):
             d = grad_out.new_empty(ctx.table)
-        return _embed_backward(grad_out, tokens.contiguous(), d, ctx.scale, ctx.padding, False), None, None, None
+            return _embed_backward(grad_out, tokens, d, ctx.scale, ctx.padding, False), None, None, None
 
 
 def embed_tokens(weight, tokens, scale=1.0, padding_idx=None):
@@ -309,7 +308,8 @@ def embed_tokens_backward(grad_out, tokens, grad_weight, scale=1.0, padding_idx=
     tokens = _token_tensor(tokens, dev)
     if grad_out.shape != tokens.shape + (grad_weight.shape[1],):
         raise RuntimeError("grad_out must be [..., H] for tokens [...] and grad_weight [V, H]")
-    _embed_backward(grad_out.detach(), tokens, grad_weight.detach(), scale, padding, accumulate)
+    with _on(dev):
+        _embed_backward(grad_out.detach(), tokens, grad_weight.detach(), scale, padding, accumulate)
     torch.autograd.graph.increment_version(grad_weight)  # written in place: autograd's checks see it
     return grad_weight
 

@@ -438,10 +438,19 @@ def test_embedding_gradient_of_sorted_sets(voc, ops):
     for t in ([7] * 999, [0] * 100, list(range(499, -1, -1)), [5, -1, 500, 5, 1 << 40, 0, 499] * 31, [3] * 16 + [4] * 16 + [5] * 32 + [6],
               [1] + [9] * 63 + [2], [498] * 17 + [499] * 47):
         t = torch.tensor(t, device="cuda")
-        g = torch.randn((len(t), H), device="cuda")
-        for at in (t, t.flip(0)):
-            _check_grad(voc, g, at, V, 2.0, 0)
+        for at in (t, t.flip(0), t.repeat(16), t.repeat_interleave(16), t.repeat_interleave(9).flip(0)):  # few positions, and many
+            _check_grad(voc, torch.randn((len(at), H), device="cuda"), at, V, 2.0, 0)
     assert ops.read_status() == 4
+
+
+@gpu
+@pytest.mark.parametrize("n", [255, 256, 257, 1023, 1024, 1025, 2049, 8191, 33000])
+def test_embedding_gradient_around_the_kernels_limits(voc, n):
+    """One position more or less than a launch, a tile or a piece holds; a table beyond one window of a bucket's tokens."""
+    for V, H in ((7, 5), (1025, 33), (140_001, 8)):
+        t = torch.randint(0, V, (n,), device="cuda")
+        t[: n // 3] = V - 1
+        _check_grad(voc, torch.randn((n, H), device="cuda").half(), t, V, 1.5, 0, torch.float32)
 
 
 @gpu
