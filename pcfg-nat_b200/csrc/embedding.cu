@@ -390,6 +390,8 @@ __global__ void __launch_bounds__(32 * kSumWarps)
     embed_sum_kernel(const G *__restrict__ grad, int64_t g_stride, int H, Pieces p, W *dw, int64_t dw_stride, float scale,
                      int accumulate) {
     constexpr int kCols = kColumns<G>, kMine = kCols / 32;
+    constexpr int kUnit = 16 / sizeof(W) < kMine ? 16 / sizeof(W) : kMine;  // columns side by side: one store of the table's type
+    const auto column = [](int k, int lane) { return ALIGNED ? k / kUnit * (32 * kUnit) + lane * kUnit + k % kUnit : k * 32 + lane; };
     __shared__ __align__(16) G staged[kSumWarps][kAhead][kCols];
     __shared__ float crossing[kSumWarps][2][kCols];
     __shared__ int4 ends[kSumWarps];  // of a warp's share: first and last token, whether those runs go on before and behind it
@@ -423,13 +425,16 @@ __global__ void __launch_bounds__(32 * kSumWarps)
             __syncwarp();
             const G *row = staged[warp][slot];
             if constexpr (ALIGNED) {
-                float x[kMine];
-                unpack_vec<G, kMine>(*reinterpret_cast<const uint4 *>(row + kMine * lane), x);
 #pragma unroll
-                for (int k = 0; k < kMine; k++) acc[k] += x[k];
+                for (int k = 0; k < kMine; k += kUnit) {
+                    float x[kUnit];
+                    unpack_vec<G, kUnit>(*reinterpret_cast<const typename RawVec<kUnit * sizeof(G)>::type *>(row + column(k, lane)), x);
+#pragma unroll
+                    for (int q = 0; q < kUnit; q++) acc[k + q] += x[q];
+                }
             } else {
 #pragma unroll
-                for (int k = 0; k < kMine; k++) acc[k] += num_to_float<G>(row[k * 32 + lane]);
+                for (int k = 0; k < kMine; k++) acc[k] += num_to_float<G>(row[column(k, lane)]);
             }
             __syncwarp();  // the row has been read
             const int ahead = i + kAhead;
@@ -451,14 +456,15 @@ __global__ void __launch_bounds__(32 * kSumWarps)
             if (began_before || goes_on) {
                 float *to = crossing[warp][began_before ? 0 : 1];
 #pragma unroll
-                for (int k = 0; k < kMine; k++) to[ALIGNED ? kMine * lane + k : k * 32 + lane] = acc[k];
-            } else if constexpr (ALIGNED) {
-                if (kMine * lane < columns) write_row<W, kMine>(dw + run * dw_stride + tile + kMine * lane, acc, scale, accumulate);
+                for (int k = 0; k < kMine; k++) to[column(k, lane)] = acc[k];
             } else {
+                constexpr int kStore = ALIGNED ? kUnit : 1;
 #pragma unroll
-                for (int k = 0; k < kMine; k++) {
-                    const float one[1] = {acc[k]};
-                    if (k * 32 + lane < columns) write_row<W, 1>(dw + run * dw_stride + tile + k * 32 + lane, one, scale, accumulate);
+                for (int k = 0; k < kMine; k += kStore) {
+                    float x[kStore];
+#pragma unroll
+                    for (int q = 0; q < kStore; q++) x[q] = acc[k + q];
+                    if (column(k, lane) < columns) write_row<W, kStore>(dw + run * dw_stride + tile + column(k, lane), x, scale, accumulate);
                 }
             }
 #pragma unroll

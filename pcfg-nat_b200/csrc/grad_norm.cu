@@ -12,8 +12,9 @@ namespace pcfgnat {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBlocksPerSm = 4;
+constexpr int kBlocksPerSm = 8;      // base model, halves to floats: 98 us, with four 115
 constexpr int kChunk = 8192;        // numbers that a block takes at a time
+constexpr int kUnroll = 4;           // loads of a thread in flight
 constexpr int kMaxTensors = 1024;   // of one launch: 29 bytes each of the 32 764 that parameters may have
 
 // N is a few sizes, so that a short list does not pay for the parameters of a long one.
@@ -103,12 +104,12 @@ __global__ void __launch_bounds__(kThreads) grad_squares_kernel(const __grid_con
             const RowCut<T> cut(src, n);
             const uint4 *vec = reinterpret_cast<const uint4 *>(src + cut.head);
             int i = tid;
-            for (; i + 3 * kThreads < cut.vecs; i += 4 * kThreads) {
-                uint4 raw[4];
+            for (; i + (kUnroll - 1) * kThreads < cut.vecs; i += kUnroll * kThreads) {
+                uint4 raw[kUnroll];
 #pragma unroll
-                for (int j = 0; j < 4; j++) raw[j] = __ldg(vec + i + j * kThreads);
+                for (int j = 0; j < kUnroll; j++) raw[j] = __ldg(vec + i + j * kThreads);
 #pragma unroll
-                for (int j = 0; j < 4; j++) sum += squares<T>(raw[j]);
+                for (int j = 0; j < kUnroll; j++) sum += squares<T>(raw[j]);
             }
             for (; i < cut.vecs; i += kThreads) sum += squares<T>(__ldg(vec + i));
             if (tid < cut.loose(n)) {
@@ -147,26 +148,31 @@ __global__ void __launch_bounds__(kThreads)
             const T *src = static_cast<const T *>(t.src[k]) + begin;
             const auto write = [&](auto other) {
                 using D = decltype(other);
-                constexpr int kVec = 16 / sizeof(T);
+                // whole 16-byte stores side by side: halves are read eight bytes at a time where floats are written
+                constexpr int kNum = 16 / sizeof(D);
+                using Raw = typename RawVec<kNum * sizeof(T)>::type;
                 D *dst = static_cast<D *>(t.dst[k]) + begin;
                 const RowCut<T> cut(src, n);
-                const uint4 *vec = reinterpret_cast<const uint4 *>(src + cut.head);
+                const Raw *from = reinterpret_cast<const Raw *>(src + cut.head);
                 if (!(reinterpret_cast<uintptr_t>(dst + cut.head) & 15)) {
-                    for (int i = tid; i < cut.vecs; i += kThreads) {
-                        float x[kVec];
-                        unpack_vec<T, kVec>(vec[i], x);
+                    const auto scale_vector = [&](const Raw &raw, int i) {
+                        float x[kNum];
+                        unpack_vec<T, kNum>(raw, x);
 #pragma unroll
-                        for (int j = 0; j < kVec; j++) x[j] *= factor;
+                        for (int j = 0; j < kNum; j++) x[j] *= factor;
+                        // not read again here: it should not push out what is still to be read
+                        __stcs(reinterpret_cast<uint4 *>(dst + cut.head) + i, pack_vec<D, kNum>(x));
+                    };
+                    const int units = cut.vecs * RowCut<T>::kVec / kNum;
+                    int i = tid;
+                    for (; i + (kUnroll - 1) * kThreads < units; i += kUnroll * kThreads) {
+                        Raw raw[kUnroll];
 #pragma unroll
-                        for (int j = 0; j < kVec; j += 16 / sizeof(D)) {
-                            constexpr int kOut = 16 / sizeof(D) < kVec ? 16 / sizeof(D) : kVec;
-                            float y[kOut];
+                        for (int j = 0; j < kUnroll; j++) raw[j] = from[i + j * kThreads];
 #pragma unroll
-                            for (int q = 0; q < kOut; q++) y[q] = x[j + q];
-                            // not read again here: it should not push out what is still to be read
-                            __stcs(reinterpret_cast<uint4 *>(dst + cut.head + i * kVec + j), pack_vec<D, kOut>(y));
-                        }
+                        for (int j = 0; j < kUnroll; j++) scale_vector(raw[j], i + j * kThreads);
                     }
+                    for (; i < units; i += kThreads) scale_vector(from[i], i);
                     if (tid < cut.loose(n)) {
                         const int i = cut.loose_at(tid);
                         dst[i] = num_from_float<D>(num_to_float<T>(src[i]) * factor);
