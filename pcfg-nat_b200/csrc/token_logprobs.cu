@@ -332,7 +332,7 @@ __device__ __forceinline__ uint32_t maximum_of(const Stats &a) { return a.s > 0.
 // Blocks that fit an SM.  More hide more of the memory's latency until their registers run out: with 40 000 numbers a row,
 // float32 rows 61, 51 and 56 us with 9, 10 and 12 blocks, halves 57, 57 and 60 us for 2 272 rows with eight alternatives.
 template <typename T, int NT>
-constexpr int kResident = NT == 512 ? 2 : NT == 32 || sizeof(T) == 4 ? 10 : 9;
+constexpr int kResident = NT == 256 ? 4 : NT == 32 || sizeof(T) == 4 ? 10 : 9;
 
 // A team of NT threads per row or, in a cluster, per part of a row; the first block of a cluster joins the parts.
 template <typename T, int NT, bool ENTROPY>
@@ -520,13 +520,15 @@ int launch_token_logprobs(const void *logits, int dtype, int64_t n, int64_t inne
             return cuda_rc(entropy ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT, true>, rows, n, given, out)
                                    : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT, false>, rows, n, given, out));
         };
-        // A warp per row while a lane has no more than eight vectors; else a block of 128 threads, and up to eight blocks per row
-        // where the rows alone do not fill the GPU and every thread of them still has two vectors.
+        // A warp per row while a lane has no more than eight vectors.  A block of 128 threads where many rows keep every SM busy, or
+        // a row is over in a few loads; one of 256 for fewer rows (64 rows of 40 000 halves 8.2 against 10.2 us), and up to eight
+        // of them where a thread would see more than twenty vectors (64 rows of 128 256: 14.3 against 18.4 us) while that fills no
+        // more than the GPU: a cluster costs two barriers (64 rows of 40 000 by clusters of two: 10.2 us).
         if (vecs <= 256) return run(std::integral_constant<int, 32>(), 1);
+        if (n > 2 * sms || vecs <= 1024) return run(std::integral_constant<int, 128>(), 1);
         int parts = 1;
-        while (parts < 8 && n * parts * 2 <= 8 * sms && vecs >= (int64_t)parts * 2 * 256) parts *= 2;
-        if (parts == 8 && n * parts <= sms && vecs >= 8 * 1024) return run(std::integral_constant<int, 512>(), parts);
-        return run(std::integral_constant<int, 128>(), parts);
+        while (parts < 8 && vecs > (int64_t)parts * 20 * 256 && n * parts * 2 <= 2 * sms) parts *= 2;
+        return run(std::integral_constant<int, 256>(), parts);
     });
 }
 
