@@ -395,22 +395,25 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, kResident<T, NT>)
     if (warp == 0) write_out<NT, ENTROPY>(out, t, a, r, inside, x_token, lane);
 }
 
-constexpr int kThreads = 256;
-
 // d x_v = p_v (-G - h (log p_v + H)) + sum of the gradients given to v, G their sum over the row, h the entropy's.
 // The few entries that tokens and alternatives name are formed again, with what is added, before they are rounded.
-// A block per row, or per part of a row (blockIdx.y) where the rows alone do not fill the GPU.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    token_logprobs_grad_kernel(Rows rows, Given given, int top, const float *__restrict__ kept, const float *__restrict__ entropy,
-                               const int64_t *__restrict__ top_index, const float *__restrict__ g_logprob,
-                               const float *__restrict__ g_entropy, const float *__restrict__ g_top, T *dlogits, int64_t pitch,
-                               int *status) {
-    constexpr int kVec = RowCut<T>::kVec;
-    __shared__ int at[kMaxTop + 1];
-    __shared__ float add[kMaxTop + 1];
-    const int tid = threadIdx.x;
-    const int64_t r = blockIdx.x;
+// A team of NT threads per row, or per part of a row (blockIdx.y) where the rows alone do not fill the GPU.
+template <typename T, int NT>
+constexpr int kGradAhead = NT == 512 && sizeof(T) == 2 ? 2 : 4;  // loads of a thread in flight
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT < 512 ? 12 : sizeof(T) == 2 ? 4 : 3)
+    token_logprobs_grad_kernel(Rows rows, int64_t n_rows, Given given, int top, const float *__restrict__ kept,
+                               const float *__restrict__ entropy, const int64_t *__restrict__ top_index,
+                               const float *__restrict__ g_logprob, const float *__restrict__ g_entropy,
+                               const float *__restrict__ g_top, T *dlogits, int64_t pitch, int *status) {
+    constexpr int kVec = RowCut<T>::kVec, kAhead = kGradAhead<T, NT>, kTeams = NT < 128 ? 128 / NT : 1;
+    __shared__ int all_at[kTeams][kMaxTop + 1];
+    __shared__ float all_add[kTeams][kMaxTop + 1];
+    const int tid = threadIdx.x % NT, team = kTeams == 1 ? 0 : threadIdx.x / NT;
+    int *at = all_at[team];
+    float *add = all_add[team];
+    const int64_t r = (int64_t)blockIdx.x * kTeams + team;
+    if (r >= n_rows) return;
     const int V = rows.V;
     const T *row = rows.at<T>(r);
     T *out = dlogits + r * pitch;
@@ -419,15 +422,15 @@ __global__ void __launch_bounds__(kThreads)
     const float m = kept[2 * r], log_s = kept[2 * r + 1];
     const bool bad = !left_out && g_logprob && (token < 0 || token >= V);
     if (bad && tid == 0) flag(status, PCFGNAT_STATUS_BAD_INDEX);
-    if (tid <= kMaxTop) {
+    for (int k = tid; k <= top; k += NT) {  // number 0: the token
         int64_t index = -1;
         float g = 0.f;
-        if (tid == 0 && g_logprob) index = token, g = g_logprob[r];
-        if (tid > 0 && tid <= top && g_top) index = top_index[r * top + tid - 1], g = index < 0 ? 0.f : g_top[r * top + tid - 1];
-        at[tid] = index < 0 || index >= V ? -1 : (int)index;
-        add[tid] = g;
+        if (k == 0 && g_logprob) index = token, g = g_logprob[r];
+        if (k > 0 && g_top) index = top_index[r * top + k - 1], g = index < 0 ? 0.f : g_top[r * top + k - 1];
+        at[k] = index < 0 || index >= V ? -1 : (int)index;
+        add[k] = g;
     }
-    __syncthreads();
+    team_sync<NT>();
     float G = 0.f;
     for (int k = 0; k <= top; k++) G += add[k];
     if (bad) G = CUDART_NAN_F;
@@ -464,27 +467,28 @@ __global__ void __launch_bounds__(kThreads)
     }
     uint4 *to = reinterpret_cast<uint4 *>(out + cut.head);
     if (zero) {
-        for (int i = first + tid; i < last; i += kThreads) to[i] = make_uint4(0, 0, 0, 0);
+        for (int i = first + tid; i < last; i += NT) to[i] = make_uint4(0, 0, 0, 0);
         return;
     }
     if (same) {
         const uint4 *vec = reinterpret_cast<const uint4 *>(row + cut.head);
         int i = first + tid;
-        for (; i + (kUnroll - 1) * kThreads < last; i += kUnroll * kThreads) {
-            uint4 raw[kUnroll];
+        for (; i + (kAhead - 1) * NT < last; i += kAhead * NT) {
+            uint4 raw[kAhead];
 #pragma unroll
-            for (int k = 0; k < kUnroll; k++) raw[k] = __ldg(vec + i + k * kThreads);
+            for (int k = 0; k < kAhead; k++) raw[k] = __ldg(vec + i + k * NT);
 #pragma unroll
-            for (int k = 0; k < kUnroll; k++) to[i + k * kThreads] = grad_vec(raw[k]);
+            for (int k = 0; k < kAhead; k++) to[i + k * NT] = grad_vec(raw[k]);
         }
-        for (; i < last; i += kThreads) to[i] = grad_vec(__ldg(vec + i));
+        for (; i < last; i += NT) to[i] = grad_vec(__ldg(vec + i));
     } else {  // rows that begin at different places of a 16-byte vector
-        for (int i = first * kVec + tid; i < last * kVec; i += kThreads)
+        for (int i = first * kVec + tid; i < last * kVec; i += NT)
             out[cut.head + i] = num_from_float<T>(grad(num_to_float<T>(row[cut.head + i])));
     }
-    __syncthreads();
-    if (tid <= top && at[tid] >= 0) {
-        const int i = at[tid], v = i < cut.head || i >= cut.head + cut.vecs * kVec ? -1 : (i - cut.head) / kVec;
+    team_sync<NT>();
+    for (int q = tid; q <= top; q += NT) {
+        if (at[q] < 0) continue;
+        const int i = at[q], v = i < cut.head || i >= cut.head + cut.vecs * kVec ? -1 : (i - cut.head) / kVec;
         if (v < 0 ? blockIdx.y == 0 : v >= first && v < last) {  // written by this block
             float g = 0.f;
             for (int k = 0; k <= top; k++) g += at[k] == i ? add[k] : 0.f;
@@ -541,12 +545,21 @@ int launch_token_logprobs_grad(const void *logits, int dtype, int64_t n, int64_t
     const Given given{tokens, ignore, has_ignore};
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        // parts of at least two vectors per thread while there are fewer blocks than the GPU holds at once
-        const int64_t vecs = V / RowCut<T>::kVec, room = 8 * (int64_t)sm_count() / n;
-        const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({room, vecs / (2 * kThreads), 64}));
-        token_logprobs_grad_kernel<T><<<dim3((unsigned)n, (unsigned)parts), kThreads, 0, st>>>(
-            rows, given, top, kept, entropy, top_index, g_logprob, g_entropy, g_top, static_cast<T *>(dlogits), pitch, status);
-        return cuda_rc(cudaGetLastError());
+        // A warp per row while a lane has no more than eight vectors, blocks of 128 threads up to 32 KB a row, else of 512: rows of
+        // 1 000 halves 16.5 us by warps and 22.6 by blocks, of 40 000 halves 274 and 295 us by blocks of 512 and 128 threads.
+        const int64_t vecs = V / RowCut<T>::kVec;
+        const auto run = [&](auto team) {
+            constexpr int NT = decltype(team)::value;
+            // parts of at least two vectors per thread while there are fewer threads than the GPU holds at once
+            const int64_t room = 2048 / NT * (int64_t)sm_count() / n;
+            const int64_t parts = NT < 128 ? 1 : std::max<int64_t>(1, std::min<int64_t>({room, vecs / (2 * NT), 64}));
+            token_logprobs_grad_kernel<T, NT><<<dim3((unsigned)(NT < 128 ? (n * NT + 127) / 128 : n), (unsigned)parts), NT < 128 ? 128 : NT, 0, st>>>(
+                rows, n, given, top, kept, entropy, top_index, g_logprob, g_entropy, g_top, static_cast<T *>(dlogits), pitch, status);
+            return cuda_rc(cudaGetLastError());
+        };
+        if (vecs <= 256) return run(std::integral_constant<int, 32>());
+        if (vecs <= 2048) return run(std::integral_constant<int, 128>());
+        return run(std::integral_constant<int, 512>());
     });
 }
 
