@@ -332,13 +332,13 @@ __device__ __forceinline__ uint32_t maximum_of(const Stats &a) { return a.s > 0.
 // Blocks that fit an SM.  More hide more of the memory's latency until their registers run out: with 40 000 numbers a row,
 // float32 rows 61, 51 and 56 us with 9, 10 and 12 blocks, halves 57, 57 and 60 us for 2 272 rows with eight alternatives.
 template <typename T, int NT>
-constexpr int kResident = NT == 256 ? 4 : NT == 32 || sizeof(T) == 4 ? 10 : 9;
+constexpr int kResident = NT == 256 ? 4 : NT == 64 ? 16 : NT == 32 || sizeof(T) == 4 ? 10 : 9;
 
 // A team of NT threads per row or, in a cluster, per part of a row; the first block of a cluster joins the parts.
 template <typename T, int NT, bool ENTROPY>
-__global__ void __launch_bounds__(NT < 128 ? 128 : NT, kResident<T, NT>)
+__global__ void __launch_bounds__(NT == 32 ? 128 : NT, kResident<T, NT>)
     token_logprobs_kernel(Rows rows, int64_t n_rows, Given given, Results out) {
-    constexpr int kTeams = NT < 128 ? 128 / NT : 1;
+    constexpr int kTeams = NT == 32 ? 4 : 1;
     __shared__ Team<NT> teams[kTeams];
     Team<NT> &t = teams[kTeams == 1 ? 0 : threadIdx.x / NT];
     const int tid = threadIdx.x % NT, warp = tid >> 5, lane = tid & 31;
@@ -401,12 +401,12 @@ __global__ void __launch_bounds__(NT < 128 ? 128 : NT, kResident<T, NT>)
 template <typename T, int NT>
 constexpr int kGradAhead = NT == 512 && sizeof(T) == 2 ? 2 : 4;  // loads of a thread in flight
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT < 128 ? 128 : NT, NT < 512 ? 12 : sizeof(T) == 2 ? 4 : 3)
+__global__ void __launch_bounds__(NT == 32 ? 128 : NT, NT < 512 ? 12 : sizeof(T) == 2 ? 4 : 3)
     token_logprobs_grad_kernel(Rows rows, int64_t n_rows, Given given, int top, const float *__restrict__ kept,
                                const float *__restrict__ entropy, const int64_t *__restrict__ top_index,
                                const float *__restrict__ g_logprob, const float *__restrict__ g_entropy,
                                const float *__restrict__ g_top, T *dlogits, int64_t pitch, int *status) {
-    constexpr int kVec = RowCut<T>::kVec, kAhead = kGradAhead<T, NT>, kTeams = NT < 128 ? 128 / NT : 1;
+    constexpr int kVec = RowCut<T>::kVec, kAhead = kGradAhead<T, NT>, kTeams = NT == 32 ? 4 : 1;
     __shared__ int all_at[kTeams][kMaxTop + 1];
     __shared__ float all_add[kTeams][kMaxTop + 1];
     const int tid = threadIdx.x % NT, team = kTeams == 1 ? 0 : threadIdx.x / NT;
@@ -512,8 +512,8 @@ int launch_token_logprobs(const void *logits, int dtype, int64_t n, int64_t inne
         const auto run = [&](auto team, int parts) {
             constexpr int NT = decltype(team)::value;
             cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3((unsigned)(NT < 128 ? (n * NT + 127) / 128 : n * parts));
-            cfg.blockDim = dim3(NT < 128 ? 128 : NT);
+            cfg.gridDim = dim3((unsigned)(NT == 32 ? (n * NT + 127) / 128 : n * parts));
+            cfg.blockDim = dim3(NT == 32 ? 128 : NT);
             cfg.stream = st;
             cudaLaunchAttribute attr[1];
             attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -524,11 +524,13 @@ int launch_token_logprobs(const void *logits, int dtype, int64_t n, int64_t inne
             return cuda_rc(entropy ? cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT, true>, rows, n, given, out)
                                    : cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT, false>, rows, n, given, out));
         };
-        // A warp per row while a lane has no more than eight vectors.  A block of 128 threads where many rows keep every SM busy, or
-        // a row is over in a few loads; one of 256 for fewer rows (64 rows of 40 000 halves 8.2 against 10.2 us), and up to eight
-        // of them where a thread would see more than twenty vectors (64 rows of 128 256: 14.3 against 18.4 us) while that fills no
-        // more than the GPU: a cluster costs two barriers (64 rows of 40 000 by clusters of two: 10.2 us).
+        // A warp per row while a lane has no more than eight vectors.  Where many rows keep every SM busy a block of 64 (2 000 rows of
+        // 4 096 halves 14.4 against 17.4 us by 128) or 128 threads; 128 too where a row is over in a few loads.  For fewer rows one
+        // of 256 (64 rows of 40 000 halves 8.2 against 10.2 us), and up to eight of them where a thread would see more than twenty
+        // vectors (64 rows of 128 256: 14.3 against 18.4 us) while that is no more than the GPU holds: a cluster costs two barriers
+        // (64 rows of 40 000 halves by clusters of two 10.2 us).
         if (vecs <= 256) return run(std::integral_constant<int, 32>(), 1);
+        if (n > 2 * sms && vecs <= 1024) return run(std::integral_constant<int, 64>(), 1);
         if (n > 2 * sms || vecs <= 1024) return run(std::integral_constant<int, 128>(), 1);
         int parts = 1;
         while (parts < 8 && vecs > (int64_t)parts * 20 * 256 && n * parts * 2 <= 2 * sms) parts *= 2;
@@ -552,8 +554,8 @@ int launch_token_logprobs_grad(const void *logits, int dtype, int64_t n, int64_t
             constexpr int NT = decltype(team)::value;
             // parts of at least two vectors per thread while there are fewer threads than the GPU holds at once
             const int64_t room = 2048 / NT * (int64_t)sm_count() / n;
-            const int64_t parts = NT < 128 ? 1 : std::max<int64_t>(1, std::min<int64_t>({room, vecs / (2 * NT), 64}));
-            token_logprobs_grad_kernel<T, NT><<<dim3((unsigned)(NT < 128 ? (n * NT + 127) / 128 : n), (unsigned)parts), NT < 128 ? 128 : NT, 0, st>>>(
+            const int64_t parts = NT == 32 ? 1 : std::max<int64_t>(1, std::min<int64_t>({room, vecs / (2 * NT), 64}));
+            token_logprobs_grad_kernel<T, NT><<<dim3((unsigned)(NT == 32 ? (n * NT + 127) / 128 : n), (unsigned)parts), NT == 32 ? 128 : NT, 0, st>>>(
                 rows, n, given, top, kept, entropy, top_index, g_logprob, g_entropy, g_top, static_cast<T *>(dlogits), pitch, status);
             return cuda_rc(cudaGetLastError());
         };
