@@ -442,7 +442,8 @@ int pcfgnat_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t 
                            float *logprob, float *entropy, float *top_logprob, int64_t *top_index, float *kept, int *status,
                            void *stream);
 /* The gradient of the logits, in their type, every cell of d_logits [rows][pitch] up to V (pitch >= V; what lies behind V stays
- * as it is).  grad_logprob [rows], grad_entropy [rows] (with the forward's entropy) and grad_top [rows][top] (with its
+ * as it is), which must not overlap the logits; fastest where every row of it begins at the same place of a 16-byte vector as the
+ * logits' row.  grad_logprob [rows], grad_entropy [rows] (with the forward's entropy) and grad_top [rows][top] (with its
  * top_index) may each be NULL.  Rows that were left out, and rows of nothing but -inf, get zeros; a row whose token is out of
  * range gets NaN when grad_logprob is given. */
 int pcfgnat_token_logprobs_backward(const void *logits, int dtype, int64_t rows, int64_t rows_inner, int64_t stride_outer,
@@ -458,7 +459,8 @@ int pcfgnat_embed(const void *weight, int dtype, int64_t weight_stride, int64_t 
 /* The table's gradient: row v of d_weight [V] (grad_stride, d_stride: numbers between rows) = scale * the sum of grad_out's rows
  * whose token is v, in float32 and in an order that the tokens alone decide.  Tokens equal to padding_idx (with has_padding) and
  * tokens out of range (flagged) count for nothing.  d_dtype is PCFGNAT_DTYPE_F32 or grad_out's dtype.  accumulate: added onto the
- * rows that occur, the others stay as they are; otherwise every row is written.  n < 2^31. */
+ * rows that occur, the others stay as they are; otherwise every row is written.  Positions that count for nothing are not read
+ * in grad_out.  n, V < 2^31, H <= 2^20. */
 size_t pcfgnat_embed_backward_workspace_bytes(int64_t n, int64_t V, int H);
 int pcfgnat_embed_backward(const void *grad_out, int dtype, int64_t grad_stride, const int64_t *tokens, int64_t n, int64_t V,
                            int H, float scale, int has_padding, int64_t padding_idx, void *d_weight, int d_dtype,
@@ -470,7 +472,7 @@ int pcfgnat_embed_backward(const void *grad_out, int dtype, int64_t grad_stride,
  * itself (left alone where c * grad_scale is 1) or memory that overlaps no other tensor (PCFGNAT_ERR_INVALID_ARGUMENT
  * otherwise); dst_dtype[i] is src_dtype[i] or PCFGNAT_DTYPE_F32.  The arrays are host memory and are read before the call
  * returns; sums are held in float64 and do not depend on timing.  A norm of NaN makes every output NaN; an infinite one makes them
- * 0, and NaN where the gradient is infinite or NaN. */
+ * 0, and NaN where the gradient is infinite or NaN; an infinite max_norm means c = 1 whatever the norm. */
 size_t pcfgnat_clip_grad_norm_workspace_bytes(int n);
 int pcfgnat_clip_grad_norm(int n, const void *const *src, const int *src_dtype, void *const *dst, const int *dst_dtype,
                            const int64_t *size, float max_norm, float grad_scale, void *workspace, size_t workspace_bytes,

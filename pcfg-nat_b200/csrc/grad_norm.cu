@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kThreads)
     sum = block_sum(sum, part);
     const float norm = (float)(fabs((double)scale) * sqrt(sum));
     if (norm_out && blockIdx.x == 0 && tid == 0) *norm_out = norm;
-    const float part_of = limit / (norm + 1e-6f);
+    const float part_of = limit == CUDART_INF_F ? 1.f : limit / (norm + 1e-6f);  // no limit: whatever the norm is
     const float factor = (part_of >= 1.f ? 1.f : part_of) * scale;  // NaN stays NaN
     if (factor == 1.f && t.all_in_place) return;
     for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {  // what was read last is still in L2

@@ -126,8 +126,8 @@ def _rows(t):
 
 
 def _logits_rows(logits):
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise RuntimeError("logits must be [..., V] with V >= 1")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] < 1 << 31:
+        raise RuntimeError("logits must be [..., V] with V >= 1, below 2^31")
     if logits.shape[-1] > 1 and logits.stride(-1) != 1:
         raise RuntimeError("the vocabulary must be the dimension of stride 1 of logits")
     rows = _rows(logits)
@@ -217,8 +217,8 @@ def token_logprobs(logits, tokens, top=0, entropy=False, ignore_index=None):
 
 def _table(weight, name):
     dt = _numbers(weight, name)
-    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise RuntimeError(f"{name} must be [V, H]")
+    if weight.dim() != 2 or not 1 <= weight.shape[0] < 1 << 31 or not 1 <= weight.shape[1] <= 1 << 20:
+        raise RuntimeError(f"{name} must be [V, H] with 1 <= V < 2^31 and 1 <= H <= 2^20")
     if weight.shape[1] > 1 and weight.stride(1) != 1 or weight.shape[0] > 1 and weight.stride(0) < weight.shape[1]:
         raise RuntimeError(f"the rows of {name} must be contiguous and apart")
     return dt
@@ -336,7 +336,7 @@ def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
     tensors of one device, float32, float16 or bfloat16 mixed, any number of them, in any dense layout; None among them is skipped
     (with its output).  Returns the norm before clipping, a float32 tensor on the device; nothing is read back.
 
-    ``max_norm=math.inf`` only measures and scales; 0 makes every gradient 0.  Squares are summed in float64, in an order that the
+    ``max_norm=math.inf`` only measures and scales by ``grad_scale``, whatever the norm; 0 makes every gradient 0.  Squares are summed in float64, in an order that the
     sizes alone decide.  A norm of NaN makes every gradient NaN; an infinite one makes finite gradients 0."""
     _ops._require_cuda()
     max_norm = float(max_norm)
@@ -353,9 +353,9 @@ def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
     try:
         at = list(map(torch.Tensor.data_ptr, every))
     except TypeError:
-        if any(g is not None and not isinstance(g, torch.Tensor) for g in every):
-            raise RuntimeError("gradients and outputs must be tensors") from None
         there = [i for i, g in enumerate(grads) if g is not None]
+        if len(there) == len(grads):  # not because of a gradient that is None
+            raise RuntimeError("gradients and outputs must be tensors") from None
         grads = [grads[i] for i in there]
         return clip_grad_norm_(grads, max_norm, None if out is None else [outs[i] for i in there], grad_scale)
     n = len(grads)

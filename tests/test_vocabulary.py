@@ -482,6 +482,18 @@ def test_embedding_gradient_through_autograd_and_of_broadcast_gradients(voc):
 
 
 @gpu
+@pytest.mark.parametrize("n", [100, 3000])
+def test_embedding_gradient_of_padding_is_not_read(voc, n):
+    t = torch.randint(0, 50, (n,), device="cuda")
+    t[::3], t[1::7] = 4, -5
+    g = torch.randn((n, 24), device="cuda")
+    g[(t == 4) | (t < 0)] = math.nan
+    want, room = _grad64(torch.where(torch.isnan(g), 0, g), t, 50, 1.0, 4)
+    d = voc.embed_tokens_backward(g, t, torch.empty((50, 24), device="cuda"), padding_idx=4, accumulate=False)
+    _close(d, want, room)
+
+
+@gpu
 def test_embedding_gradient_against_differences(voc):
     w = torch.randn((20, 7), device="cuda", requires_grad=True)
     t = torch.randint(0, 20, (33,), device="cuda")
@@ -570,6 +582,8 @@ def test_clipping_of_extreme_and_non_finite_gradients(voc):
         assert abs(float(norm) - want) <= 4 * U * want
     for bad in (math.nan, math.inf):
         g = [torch.ones(10, device="cuda"), torch.tensor([1.0, bad], device="cuda")]
+        norm = voc.clip_grad_norm_(g, math.inf)  # measured only
+        assert not math.isfinite(float(norm)) and torch.equal(g[0], torch.ones(10, device="cuda")) and g[1][0] == 1
         norm = voc.clip_grad_norm_(g, 1.0)
         assert math.isnan(float(norm)) if math.isnan(bad) else float(norm) == math.inf
         if math.isnan(bad):
@@ -834,6 +848,7 @@ def test_refusals(voc):
         (lambda: voc.token_logprobs(x[:, :0], t), "V >= 1"),
         (lambda: voc.embed_tokens(x, t.float()), "int64"),
         (lambda: voc.embed_tokens(x[0], t), r"\[V, H\]"),
+        (lambda: voc.embed_tokens(x[:, :0], t), r"\[V, H\]"),
         (lambda: voc.embed_tokens(x[:1].expand(4, 8), t), "apart"),
         (lambda: voc.embed_tokens_backward(x, t, torch.zeros((5, 7), device="cuda")), "grad_out must be"),
         (lambda: voc.embed_tokens_backward(x.half(), t, torch.zeros((5, 8), device="cuda").bfloat16()), "grad_weight must be"),
@@ -841,6 +856,9 @@ def test_refusals(voc):
         (lambda: voc.clip_grad_norm_([x], 1.0, out=[x[:1]]), "shape"),
         (lambda: voc.clip_grad_norm_([x], 1.0, out=[x.half()]), "type or float32"),
         (lambda: voc.clip_grad_norm_([x], 1.0, out=[]), "one tensor per gradient"),
+        (lambda: voc.clip_grad_norm_([x], 1.0, out=[None]), "must be tensors"),
+        (lambda: voc.clip_grad_norm_([x, 3.0], 1.0), "must be tensors"),
+        (lambda: voc.clip_grad_norm_([x, t.float().cpu()], 1.0), "on one device"),
         (lambda: voc.clip_grad_norm_([x[:, ::2]], 1.0), "dense"),
         (lambda: voc.clip_grad_norm_([x[:1].expand(3, 8)], 1.0), "dense"),
         (lambda: voc.clip_grad_norm_([x], -1.0), "max_norm"),
