@@ -460,7 +460,7 @@ int pcfgnat_embed(const void *weight, int dtype, int64_t weight_stride, int64_t 
  * whose token is v, in float32 and in an order that the tokens alone decide.  Tokens equal to padding_idx (with has_padding) and
  * tokens out of range (flagged) count for nothing.  d_dtype is PCFGNAT_DTYPE_F32 or grad_out's dtype.  accumulate: added onto the
  * rows that occur, the others stay as they are; otherwise every row is written.  Positions that count for nothing are not read
- * in grad_out.  n, V < 2^31, H <= 2^20. */
+ * in grad_out.  n, V < 2^31, H <= 2^20.  A few positions need no workspace: 0 bytes, which may be NULL. */
 size_t pcfgnat_embed_backward_workspace_bytes(int64_t n, int64_t V, int H);
 int pcfgnat_embed_backward(const void *grad_out, int dtype, int64_t grad_stride, const int64_t *tokens, int64_t n, int64_t V,
                            int H, float scale, int has_padding, int64_t padding_idx, void *d_weight, int d_dtype,

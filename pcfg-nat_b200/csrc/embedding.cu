@@ -297,19 +297,20 @@ __global__ void __launch_bounds__(kSortThreads, 2)
         __syncthreads();
         over([&](uint2 entry) {
             const int row = row_of(entry);
-            for (uint32_t todo = __ballot_sync(0xffffffffu, row >= 0); todo;) {  // one token after the other
-                const int one = __shfl_sync(0xffffffffu, row, __ffs(todo) - 1);
-                const uint32_t same = __ballot_sync(0xffffffffu, row == one);
-                const int from = mine[one];
-                __syncwarp();
-                if (lane == 0) mine[one] = from + __popc(same);
-                if (row == one) {
-                    const int at = from + __popc(same & ((1u << lane) - 1));
-                    sorted.token[at] = ((one + r0) << kBucketBits) + bucket, sorted.at[at] = (int)entry.y;
-                }
-                __syncwarp();
-                todo &= ~same;
+            const uint32_t in = __ballot_sync(0xffffffffu, row >= 0);
+            if (!in) return;
+            const int one = __shfl_sync(0xffffffffu, row, __ffs(in) - 1);
+            uint32_t same = __ballot_sync(0xffffffffu, row == one);  // a frequent token fills whole groups
+            if (same != in) same = __match_any_sync(0xffffffffu, row);
+            int from = 0;
+            if (row >= 0) from = mine[row];
+            __syncwarp();
+            if (row >= 0) {
+                const int rank = __popc(same & ((1u << lane) - 1)), at = from + rank;
+                if (rank == 0) mine[row] = from + __popc(same);
+                sorted.token[at] = ((row + r0) << kBucketBits) + bucket, sorted.at[at] = (int)entry.y;
             }
+            __syncwarp();
         });
         __syncthreads();
     }
@@ -689,7 +690,7 @@ struct Scratch {
 
 }  // namespace
 
-size_t embed_workspace_bytes(int64_t n, int64_t V, int H) { return n <= kFew ? 16 : Scratch(nullptr, n, V, H).bytes; }
+size_t embed_workspace_bytes(int64_t n, int64_t V, int H) { return n <= kFew ? 0 : Scratch(nullptr, n, V, H).bytes; }
 
 int launch_embed(const void *weight, int dtype, int64_t w_stride, int64_t V, int H, const int64_t *tokens, int64_t n, float scale,
                  void *out, int *status, cudaStream_t st) {

@@ -128,6 +128,8 @@ def _rows(t):
 def _logits_rows(logits):
     if logits.dim() < 1 or not 1 <= logits.shape[-1] < 1 << 31:
         raise RuntimeError("logits must be [..., V] with V >= 1, below 2^31")
+    if logits.is_contiguous():
+        return logits.numel() // logits.shape[-1] or 1, 0, logits.shape[-1]
     if logits.shape[-1] > 1 and logits.stride(-1) != 1:
         raise RuntimeError("the vocabulary must be the dimension of stride 1 of logits")
     rows = _rows(logits)
@@ -216,12 +218,16 @@ def token_logprobs(logits, tokens, top=0, entropy=False, ignore_index=None):
 
 
 def _table(weight, name):
+    """(PCFGNAT_DTYPE_*, V, H, numbers between rows) of a table."""
     dt = _numbers(weight, name)
-    if weight.dim() != 2 or not 1 <= weight.shape[0] < 1 << 31 or not 1 <= weight.shape[1] <= 1 << 20:
+    shape = weight.shape
+    if len(shape) != 2 or not 1 <= shape[0] < 1 << 31 or not 1 <= shape[1] <= 1 << 20:
         raise RuntimeError(f"{name} must be [V, H] with 1 <= V < 2^31 and 1 <= H <= 2^20")
-    if weight.shape[1] > 1 and weight.stride(1) != 1 or weight.shape[0] > 1 and weight.stride(0) < weight.shape[1]:
+    V, H = shape
+    apart, beside = weight.stride()
+    if H > 1 and beside != 1 or V > 1 and apart < H:
         raise RuntimeError(f"the rows of {name} must be contiguous and apart")
-    return dt
+    return dt, V, H, max(apart, H)
 
 
 def _finite(x, name):
@@ -232,20 +238,20 @@ def _finite(x, name):
 
 
 def _embed(weight, tokens, scale):
-    dt, dev = _table(weight, "weight"), weight.device
+    dt, V, H, apart = _table(weight, "weight")
+    dev = weight.device
     tokens = _token_tensor(tokens, dev)
-    V, H = weight.shape
     with _on(dev):
         out = weight.new_empty(tokens.shape + (H,))
-        rc = _cabi.lib().pcfgnat_embed(weight.data_ptr(), dt, weight.stride(0), V, H, tokens.data_ptr(), tokens.numel(), scale,
-                                       out.data_ptr(), _status_of(dev), _stream(dev))
+        rc = _cabi.lib().pcfgnat_embed(weight.data_ptr(), dt, apart, V, H, tokens.data_ptr(), tokens.numel(), scale, out.data_ptr(),
+                                       _status_of(dev), _stream(dev))
     _cabi.check(rc, "pcfgnat_embed")
     return out
 
 
-def _embed_backward(g, tokens, d_weight, scale, padding, accumulate):  # on the tensors' device
+def _embed_backward(g, tokens, d_weight, table, scale, padding, accumulate):  # on the tensors' device; table: as _table tells
     dev = g.device
-    V, H = d_weight.shape
+    dt, V, H, apart = table
     n = tokens.numel()
     stride = H
     if not g.is_contiguous():
@@ -255,11 +261,10 @@ def _embed_backward(g, tokens, d_weight, scale, padding, accumulate):  # on the 
         else:
             stride = rows[2]
     lib = _cabi.lib()
-    nbytes = lib.pcfgnat_embed_backward_workspace_bytes(n, V, H)
-    ws = tokens.new_empty(nbytes, dtype=torch.uint8)
+    nbytes = lib.pcfgnat_embed_backward_workspace_bytes(n, V, H)  # none for few positions
+    ws = tokens.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     rc = lib.pcfgnat_embed_backward(g.data_ptr(), _DTYPES[g.dtype], stride, tokens.data_ptr(), n, V, H, scale, *padding, d_weight.data_ptr(),
-                                    _DTYPES[d_weight.dtype], max(d_weight.stride(0), H), int(accumulate), ws.data_ptr(), nbytes,
-                                    _status_of(dev), _stream(dev))
+                                    dt, apart, int(accumulate), ws.data_ptr() if nbytes else None, nbytes, _status_of(dev), _stream(dev))
     _cabi.check(rc, "pcfgnat_embed_backward")
     return d_weight
 
@@ -269,7 +274,8 @@ class EmbedTokensFunc(Function):
     def forward(ctx, weight, tokens, scale, padding):
         out = _embed(weight, tokens, scale)  # checks them
         ctx.save_for_backward(tokens.contiguous())
-        ctx.scale, ctx.padding, ctx.table = scale, padding, weight.shape
+        V, H = ctx.shape = weight.shape
+        ctx.scale, ctx.padding, ctx.table = scale, padding, (_DTYPES[weight.dtype], V, H, H)  # the gradient's, which is contiguous
         return out
 
     @staticmethod
@@ -277,8 +283,8 @@ class EmbedTokensFunc(Function):
     def backward(ctx, grad_out):
         (tokens,) = ctx.saved_tensors
         with _on(grad_out.device):
-            d = grad_out.new_empty(ctx.table)
-            return _embed_backward(grad_out, tokens, d, ctx.scale, ctx.padding, False), None, None, None
+            d = grad_out.new_empty(ctx.shape)
+            return _embed_backward(grad_out, tokens, d, ctx.table, ctx.scale, ctx.padding, False), None, None, None
 
 
 def embed_tokens(weight, tokens, scale=1.0, padding_idx=None):
@@ -299,7 +305,7 @@ def embed_tokens_backward(grad_out, tokens, grad_weight, scale=1.0, padding_idx=
     completes without a second dense tensor.  Rows whose token does not occur are not touched.  ``accumulate=False``: every row is
     overwritten.  ``grad_weight`` is float32 or of ``grad_out``'s type."""
     _numbers(grad_out, "grad_out")
-    _table(grad_weight, "grad_weight")
+    table = _table(grad_weight, "grad_weight")
     scale = _finite(scale, "scale")
     padding = _optional_index(padding_idx, "padding_idx")
     dev = grad_out.device
@@ -309,7 +315,7 @@ def embed_tokens_backward(grad_out, tokens, grad_weight, scale=1.0, padding_idx=
     if grad_out.shape != tokens.shape + (grad_weight.shape[1],):
         raise RuntimeError("grad_out must be [..., H] for tokens [...] and grad_weight [V, H]")
     with _on(dev):
-        _embed_backward(grad_out.detach(), tokens, grad_weight.detach(), scale, padding, accumulate)
+        _embed_backward(grad_out.detach(), tokens, grad_weight.detach(), table, scale, padding, accumulate)
     torch.autograd.graph.increment_version(grad_weight)  # written in place: autograd's checks see it
     return grad_weight
 

@@ -780,8 +780,9 @@ def test_library_refuses_bad_arguments(lib):
     assert lib.pcfgnat_embed(at, 0, 4, 0, 4, at, 1, 1.0, at, None, None) == -1
     assert lib.pcfgnat_embed(None, 0, 4, 4, 4, at, 1, 1.0, at, None, None) == -1
     assert lib.pcfgnat_embed(at, 3, 4, 4, 4, at, 1, 1.0, at, None, None) == -2
-    need = lib.pcfgnat_embed_backward_workspace_bytes(10, 4, 4)
-    e = lambda dtype=1, into=0, n=10, ws=need, d=at, stride=4: lib.pcfgnat_embed_backward(
+    need = lib.pcfgnat_embed_backward_workspace_bytes(1000, 4, 4)
+    assert need > 0 and lib.pcfgnat_embed_backward_workspace_bytes(10, 4, 4) == 0
+    e = lambda dtype=1, into=0, n=1000, ws=need, d=at, stride=4: lib.pcfgnat_embed_backward(
         at, dtype, 4, at, n, 4, 4, 1.0, 0, 0, d, into, stride, 0, at, ws, None, None)
     assert e(d=None) == e(stride=3) == e(n=-1) == -1 and e(into=2) == e(dtype=3) == -2 and e(ws=need - 1) == -4 and e(n=1 << 31) == -5
 
