@@ -209,8 +209,10 @@ struct Span {
     }
 };
 
-// A block sorts a bucket by token: counted per warp and token, numbered, placed.
-__global__ void __launch_bounds__(kSortThreads, 2)
+// A block sorts a bucket by token: counted per warp and token, numbered, placed.  There are fewer buckets than SMs, so
+// that a second block per SM would only take registers away: forward and backward of 14 400 tokens on a table of 41 MB
+// take 37.6 us in all with two blocks per SM, 35.1 with one.
+__global__ void __launch_bounds__(kSortThreads, 1)
     embed_sort_kernel(int V, int tiles, int range, Sorted sorted, Zeroed zeroed) {
     extern __shared__ int cell[];  // [warp][token of the bucket]: entries of the warp's span, then where the next one goes
     __shared__ int warp_sum[kSortWarps], base;
