@@ -60,7 +60,12 @@ __global__ void __launch_bounds__(kThreads)
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kTile = 1024;           // positions that one block of the first kernel groups
 constexpr int kBucketBits = 7, kBuckets = 1 << kBucketBits;  // a bucket: the tokens v with the same v mod 128
+constexpr int kGroups = kBuckets + 1;  // of a tile: the buckets, and the token that fills much of the list
+constexpr int kChunk = kSortWarps * 32;  // tiles that a block of the second kernel goes over at a time
+constexpr int kCopyBlocks = 16;       // of the second kernel, for that token's entries
 constexpr int kMaxRange = 1024;       // tokens of a bucket that are sorted at a time
+constexpr int kFrequent = 8;          // of 32 positions that a frequent token holds
+constexpr int kManyTiles = 4;         // from here on a frequent token is looked for
 constexpr int kBatch = 4;             // entries of a lane in flight
 constexpr int kAhead = 7;             // rows that a warp has in flight
 constexpr int kShare = 8;             // entries of a warp's share are a multiple of it
@@ -94,8 +99,9 @@ struct Sorted {
     int *token, *at;     // the tokens that count and their positions, equal tokens side by side
     int *row_end;        // [V] where the list's entries of a token end
     int *total;          // entries
+    int *frequent;       // a token that fills much of the list, -1 where there is none
     uint2 *grouped;      // [tile][kTile] (token / kBuckets, position) by bucket
-    int *bucket_begin;   // [tile][kBuckets + 1] where a bucket's entries of the tile begin
+    int *bucket_begin;   // [tile][kGroups + 1] where a bucket's entries of the tile begin, the frequent token's behind them
 };
 
 struct Zeroed {  // rows [first, last) of the table that a launch's further blocks set to zero
@@ -106,12 +112,16 @@ struct Zeroed {  // rows [first, last) of the table that a launch's further bloc
     }
 };
 
-// The positions of a tile grouped by bucket, in their order within one.
+// The positions of a tile grouped by bucket, in their order within one.  A token that a quarter of 32 positions spread over the list
+// hold (every block looks at the same) is left out of its bucket, which would be sorted by one SM while the others wait, and only
+// copied by several: 28 980 tokens, half of them one, added onto a table of 512 float32 columns in 24.0 us; 36.2 while it was sorted.
 __global__ void __launch_bounds__(kTile, 2)
     embed_group_kernel(const int64_t *__restrict__ tokens, int n, int V, uint32_t padding, int tiles, Sorted sorted, Zeroed zeroed,
                        int *status) {
-    __shared__ int cell[kTile / 32][kBuckets];
-    __shared__ int begin[kBuckets], warp_sum[kBuckets / 32];
+    constexpr int kCells = (kGroups + 31) / 32 * 32;
+    __shared__ int cell[kTile / 32][kCells];
+    __shared__ int begin[kCells], warp_sum[kCells / 32];
+    __shared__ uint32_t chosen;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the next kernel waits for this one's end all the same
     if ((int)blockIdx.x >= tiles) {
         zeroed.run(blockIdx.x - tiles, gridDim.x - tiles);
@@ -120,29 +130,41 @@ __global__ void __launch_bounds__(kTile, 2)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t i = (int64_t)blockIdx.x * kTile + tid;
     const uint2 t = i < n ? reinterpret_cast<const uint2 *>(tokens)[i] : make_uint2(padding, 0);
+    uint32_t frequent = 0xffffffffu;
+    if (tiles >= kManyTiles) {
+        if (warp == 0) {
+            uint2 sample = reinterpret_cast<const uint2 *>(tokens)[(int64_t)lane * n >> 5];
+            if (sample.y != 0 || sample.x >= (uint32_t)V || sample.x == padding) sample.x = 0xffffffffu;
+            const int held = __popc(__match_any_sync(0xffffffffu, sample.x));
+            const int most = __reduce_max_sync(0xffffffffu, sample.x == 0xffffffffu ? 0 : held * 32 + lane);
+            if (most >= kFrequent * 32) frequent = __shfl_sync(0xffffffffu, sample.x, most & 31);
+            if (lane == 0) chosen = frequent;
+        }
+        __syncthreads();
+        frequent = chosen;
+    }
+    if (blockIdx.x == 0 && tid == 0) *sorted.frequent = (int)frequent;
     const bool inside = t.y == 0 && t.x < (uint32_t)V, counts = inside && t.x != padding;
     if (i < n && !inside) flag(status, PCFGNAT_STATUS_BAD_INDEX);
-    const int bucket = t.x & (kBuckets - 1);
+    const int bucket = t.x == frequent ? kBuckets : t.x & (kBuckets - 1);
     uint32_t same = __ballot_sync(0xffffffffu, counts);  // the lanes with the same bucket
 #pragma unroll
-    for (int k = 0; k < kBucketBits; k++) {
+    for (int k = 0; k <= kBucketBits; k++) {
         const uint32_t set = __ballot_sync(0xffffffffu, bucket >> k & 1);
         same &= bucket >> k & 1 ? set : ~set;
     }
 #pragma unroll
-    for (int k = 0; k < kBuckets / 32; k++) cell[warp][k * 32 + lane] = 0;
+    for (int k = 0; k < kCells / 32; k++) cell[warp][k * 32 + lane] = 0;
     __syncwarp();
     const int rank = __popc(same & ((1u << lane) - 1));
     if (counts && rank == 0) cell[warp][bucket] = __popc(same);
     __syncthreads();
-    if (tid < kBuckets) {
-        int sum = 0;
-#pragma unroll 8
-        for (int w = 0; w < kTile / 32; w++) {
-            const int c = cell[w][tid];
-            cell[w][tid] = sum;
-            sum += c;
-        }
+    if (tid < kCells) {
+        int held[kTile / 32], sum = 0;
+#pragma unroll
+        for (int w = 0; w < kTile / 32; w++) held[w] = cell[w][tid];
+#pragma unroll
+        for (int w = 0; w < kTile / 32; w++) cell[w][tid] = sum, sum += held[w];
         int scan = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -153,38 +175,42 @@ __global__ void __launch_bounds__(kTile, 2)
         begin[tid] = scan - sum;
     }
     __syncthreads();
-    if (tid < kBuckets) {
+    if (tid < kCells) {
         int before = begin[tid];
         for (int w = 0; w < warp; w++) before += warp_sum[w];
         begin[tid] = before;
-        int *out = sorted.bucket_begin + (int64_t)blockIdx.x * (kBuckets + 1);
-        out[tid] = before;
-        if (tid == 0) {
-            int all = 0;
-            for (int w = 0; w < kBuckets / 32; w++) all += warp_sum[w];
-            out[kBuckets] = all;
-        }
+        if (tid <= kGroups) sorted.bucket_begin[(int64_t)blockIdx.x * (kGroups + 1) + tid] = before;
     }
     __syncthreads();
     if (counts)
         sorted.grouped[(int64_t)blockIdx.x * kTile + begin[bucket] + cell[warp][bucket] + rank] = make_uint2(t.x >> kBucketBits, (uint32_t)i);
 }
 
-// The entries of a bucket in the tiles that one warp goes over, at most one tile per lane, numbered through.
+// The tiles that one warp goes over of up to 1 024: side by side, at most 32; where there are fewer tiles than warps, warps share one.
+struct Share {
+    int tile0, tiles, part, parts_log;
+    __device__ __forceinline__ Share(int chunk, int there, int warp) {
+        const int each = (there + kSortWarps - 1) / kSortWarps;
+        parts_log = there > 1 ? max(0, __clz(there - 1) - __clz(kSortWarps - 1)) : 31 - __clz(kSortWarps);
+        part = warp & ((1 << parts_log) - 1);
+        const int first = min((warp >> parts_log) * each, there);
+        tile0 = chunk + first, tiles = min(each, there - first);
+    }
+};
+
+// The entries of a bucket in them, at most one tile per lane, numbered through.
 struct Span {
     int begin, count, shift;  // of the lane's tile: its first number, its entries, and from a number to the place in the tiles' list
-    int n;
-    // part of parts: where there are fewer tiles than warps, several of them share one.
-    __device__ __forceinline__ Span(const Sorted &s, int bucket, int tile0, int tiles, int part, int parts, int lane, int &below) {
+    int n, tile0, tiles;
+    __device__ __forceinline__ Span(const Sorted &s, int bucket, const Share &share, int lane) : tile0(share.tile0), tiles(share.tiles) {
         int from = 0;
         count = 0;
         if (lane < tiles) {
-            const int *b = s.bucket_begin + (int64_t)(tile0 + lane) * (kBuckets + 1) + bucket;
+            const int *b = s.bucket_begin + (int64_t)(tile0 + lane) * (kGroups + 1) + bucket;
             from = b[0], count = b[1] - from;
         }
-        if (part == 0) below += from;
-        const int first = count * part / parts;
-        count = count * (part + 1) / parts - first;
+        const int first = count * share.part >> share.parts_log;
+        count = (count * (share.part + 1) >> share.parts_log) - first;
         from += first;
         begin = count;
 #pragma unroll
@@ -197,7 +223,7 @@ struct Span {
         shift = lane * kTile + from - begin;
     }
     // Entry e of them; e may differ from lane to lane, but all lanes call.
-    __device__ __forceinline__ uint2 entry(const Sorted &s, int tile0, int tiles, int e, uint2 none) const {
+    __device__ __forceinline__ uint2 entry(const Sorted &s, int e, uint2 none) const {
         int of = 0;
         if (tiles > 1) {
 #pragma unroll
@@ -209,43 +235,96 @@ struct Span {
     }
 };
 
+// The frequent token's entries behind all others, by one of several blocks, each for tiles that lie side by side.
+__device__ void copy_frequent(const Sorted &s, int tiles, int block, int *base, int *all) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int each = (tiles + kCopyBlocks - 1) / kCopyBlocks, first = min(block * each, tiles), last = min(first + each, tiles);
+    const auto range_of = [&](int tile) { return s.bucket_begin + (int64_t)tile * (kGroups + 1) + kBuckets; };
+    if (tid == 0) *all = 0;
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    int before = 0, sum = 0;
+    for (int t = tid; t < tiles; t += kSortThreads) {
+        const int *r = range_of(t);
+        before += t < first ? r[1] : r[0], sum += r[1];
+    }
+    before = __reduce_add_sync(0xffffffffu, before), sum = __reduce_add_sync(0xffffffffu, sum);
+    if (lane == 0 && sum) atomicAdd(base, before), atomicAdd(all, sum);
+    __syncthreads();
+    const int token = *s.frequent;
+    if (block == 0 && tid == 0) {
+        *s.total = *all;
+        if (token >= 0) s.row_end[token] = *all;
+    }
+    if (token < 0) return;
+    int place = *base;
+    for (int t0 = first; t0 < last; t0 += 32) {
+        int from = 0, count = 0;
+        if (t0 + lane < last) {
+            const int *r = range_of(t0 + lane);
+            from = r[0], count = r[1] - r[0];
+        }
+#pragma unroll 4
+        for (int j = 0; j < min(32, last - t0); j++) {
+            const int entries = __shfl_sync(0xffffffffu, count, j), at = __shfl_sync(0xffffffffu, from, j) + tid;
+            if (tid < entries) s.token[place + tid] = token, s.at[place + tid] = (int)s.grouped[(int64_t)(t0 + j) * kTile + at].y;
+            place += entries;
+        }
+    }
+}
+
 // A block sorts a bucket by token: counted per warp and token, numbered, placed.  There are fewer buckets than SMs, so
 // that a second block per SM would only take registers away: forward and backward of 14 400 tokens on a table of 41 MB
-// take 37.6 us in all with two blocks per SM, 35.1 with one.
+// took 37.6 us in all with two blocks per SM, 35.1 with one.
 __global__ void __launch_bounds__(kSortThreads, 1)
     embed_sort_kernel(int V, int tiles, int range, Sorted sorted, Zeroed zeroed) {
     extern __shared__ int cell[];  // [warp][token of the bucket]: entries of the warp's span, then where the next one goes
     __shared__ int warp_sum[kSortWarps], base;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (blockIdx.x >= kBuckets) {
-        zeroed.run(blockIdx.x - kBuckets, gridDim.x - kBuckets);
+    if (blockIdx.x >= kBuckets + kCopyBlocks) {
+        zeroed.run(blockIdx.x - (kBuckets + kCopyBlocks), gridDim.x - (kBuckets + kCopyBlocks));
         return;
     }
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bucket = blockIdx.x;
+    const Share share(0, min(kChunk, tiles), warp);
     if (tid == 0) base = 0;
+    if (blockIdx.x >= kBuckets) {
+        copy_frequent(sorted, tiles, blockIdx.x - kBuckets, &base, warp_sum);
+        return;
+    }
     for (int i = tid; i < kSortWarps * range; i += kSortThreads) cell[i] = 0;
     __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int frequent = *sorted.frequent;
     const int tokens = (V - bucket + kBuckets - 1) >> kBucketBits;  // of the bucket (0 where V is smaller than its number)
     const uint2 none = make_uint2(0xffffffffu, 0);
-    // A warp's tiles lie side by side, at most 32 of them; longer lists are gone over 1 024 tiles at a time.
-    const auto over = [&](auto visit) {
-        int below = 0;
-        for (int chunk = 0; chunk < tiles; chunk += kSortWarps * 32) {
-            const int there = min(kSortWarps * 32, tiles - chunk), each = (there + kSortWarps - 1) / kSortWarps;
-            const int parts = max(1, kSortWarps / there), unit = warp / parts;
-            const int tile0 = min(chunk + unit * each, tiles), mine = min(each, tiles - tile0);
-            const Span span(sorted, bucket, tile0, mine, warp % parts, parts, lane, below);
-            for (int e0 = lane; e0 - lane < span.n; e0 += 32 * kBatch) {
-                uint2 entry[kBatch];
+    // The first entries stay in registers from the count to the placing; lists of more than 1 024 tiles are gone over by as many at a time.
+    const Span head(sorted, bucket, share, lane);
+    uint2 ahead[kBatch];
 #pragma unroll
-                for (int k = 0; k < kBatch; k++) entry[k] = span.entry(sorted, tile0, mine, e0 + k * 32, none);
+    for (int k = 0; k < kBatch; k++) ahead[k] = head.entry(sorted, k * 32 + lane, none);
+    const auto rest = [&](const Span &span, int g0, auto visit) {
+        for (; g0 < span.n; g0 += 32 * kBatch) {
+            uint2 entry[kBatch];
 #pragma unroll
-                for (int k = 0; k < kBatch; k++) visit(entry[k]);
-            }
+            for (int k = 0; k < kBatch; k++) entry[k] = span.entry(sorted, g0 + k * 32 + lane, none);
+#pragma unroll
+            for (int k = 0; k < kBatch; k++)
+                if (g0 + k * 32 < span.n) visit(entry[k]);
         }
-        return below;
     };
+    const auto over = [&](auto visit) {
+#pragma unroll
+        for (int k = 0; k < kBatch; k++)
+            if (k * 32 < head.n) visit(ahead[k]);
+        rest(head, 32 * kBatch, visit);
+        for (int chunk = kChunk; chunk < tiles; chunk += kChunk)
+            rest(Span(sorted, bucket, Share(chunk, min(kChunk, tiles - chunk), warp), lane), 0, visit);
+    };
+    int below = 0;  // what the tiles hold of the buckets before this one
+    for (int t = tid; t < tiles; t += kSortThreads) below += sorted.bucket_begin[(int64_t)t * (kGroups + 1) + bucket];
+    below = __reduce_add_sync(0xffffffffu, below);
+    if (lane == 0 && below) atomicAdd(&base, below);
     int *mine = cell + warp * range;
     int begin_of_window = 0;
     for (int r0 = 0; r0 < tokens || r0 == 0; r0 += range) {  // most tables: one window of the bucket's tokens
@@ -258,24 +337,20 @@ __global__ void __launch_bounds__(kSortThreads, 1)
             const int row = (int)entry.x - r0;
             return entry.x != none.x && row >= 0 && row < rows ? row : -1;
         };
-        int below = over([&](uint2 entry) {
+        over([&](uint2 entry) {
             const int row = row_of(entry);
             const uint32_t in = __ballot_sync(0xffffffffu, row >= 0);
             const int one = __shfl_sync(0xffffffffu, row, __ffs(in) - 1);
             const uint32_t same = __ballot_sync(0xffffffffu, row == one);  // a frequent token fills whole groups
             if (row >= 0 && (row != one || lane == __ffs(in) - 1)) atomicAdd(mine + row, row == one ? __popc(same) : 1);
         });
-        if (r0 == 0) {  // what the tiles hold of the buckets before this one
-            below = __reduce_add_sync(0xffffffffu, below);
-            if (lane == 0) atomicAdd(&base, below);
-        }
         __syncthreads();
         if (r0 == 0) begin_of_window = base;
         // where every token begins, and within it every warp
-        int sum = 0;
+        int held[kSortWarps], sum = 0;
         if (tid < rows)
-#pragma unroll 8
-            for (int w = 0; w < kSortWarps; w++) sum += cell[w * range + tid];
+#pragma unroll
+            for (int w = 0; w < kSortWarps; w++) held[w] = cell[w * range + tid], sum += held[w];
         int scan = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -284,16 +359,12 @@ __global__ void __launch_bounds__(kSortThreads, 1)
         }
         if (lane == 31) warp_sum[warp] = scan;
         __syncthreads();
+        int next = begin_of_window + scan - sum + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0);
         if (tid < rows) {
-            int next = begin_of_window + scan - sum;
-            for (int w = 0; w < warp; w++) next += warp_sum[w];
-#pragma unroll 8
-            for (int w = 0; w < kSortWarps; w++) {
-                const int c = cell[w * range + tid];
-                cell[w * range + tid] = next;
-                next += c;
-            }
-            sorted.row_end[((int64_t)(r0 + tid) << kBucketBits) + bucket] = next;
+#pragma unroll
+            for (int w = 0; w < kSortWarps; w++) cell[w * range + tid] = next, next += held[w];
+            const int token = ((r0 + tid) << kBucketBits) + bucket;
+            if (token != frequent) sorted.row_end[token] = next;
         }
         begin_of_window += __reduce_add_sync(0xffffffffu, warp_sum[lane]);
         __syncthreads();
@@ -316,7 +387,6 @@ __global__ void __launch_bounds__(kSortThreads, 1)
         });
         __syncthreads();
     }
-    if (bucket == kBuckets - 1 && tid == 0) *sorted.total = begin_of_window;
 }
 
 // A finished sum into the table.  Every number of the table gets at most one sum per call, so adding to a float32 table by a
@@ -681,11 +751,12 @@ struct Scratch {
         };
         const size_t tiles = (size_t)((n + kTile - 1) / kTile);
         sorted.total = reinterpret_cast<int *>(take(sizeof(int)));
+        sorted.frequent = reinterpret_cast<int *>(take(sizeof(int)));
         sorted.token = reinterpret_cast<int *>(take((size_t)n * sizeof(int)));
         sorted.at = reinterpret_cast<int *>(take((size_t)n * sizeof(int)));
         sorted.row_end = reinterpret_cast<int *>(take((size_t)V * sizeof(int)));
         sorted.grouped = reinterpret_cast<uint2 *>(take(tiles * kTile * sizeof(uint2)));
-        sorted.bucket_begin = reinterpret_cast<int *>(take(tiles * (kBuckets + 1) * sizeof(int)));
+        sorted.bucket_begin = reinterpret_cast<int *>(take(tiles * (kGroups + 1) * sizeof(int)));
         parts = reinterpret_cast<float *>(take((size_t)piece_count(n) * 2 * H * sizeof(float)));
     }
 };
@@ -777,7 +848,7 @@ int launch_embed_backward(const void *grad, int dtype, int64_t g_stride, const i
         cfg.numAttrs = 1;
         return cudaLaunchKernelEx(&cfg, kernel, args...);
     };
-    e = launch(embed_sort_kernel, dim3(kBuckets + zeroing), kSortThreads, smem, (int)V, tiles, range, sorted, rest);
+    e = launch(embed_sort_kernel, dim3(kBuckets + kCopyBlocks + zeroing), kSortThreads, smem, (int)V, tiles, range, sorted, rest);
     if (e != cudaSuccess) return PCFGNAT_ERR_CUDA;
     const Pieces p{sorted, scratch.parts, warp_entries(n)};
     const unsigned pieces = (unsigned)piece_count(n);

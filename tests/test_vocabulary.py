@@ -454,6 +454,31 @@ def test_embedding_gradient_around_the_kernels_limits(voc, n):
 
 
 @gpu
+@pytest.mark.parametrize("n", [257, 5000, 600_000])
+@pytest.mark.parametrize("V", [1, 130, 150_000])
+@pytest.mark.parametrize("which", ["evenly", "first", "only there", "nowhere else", "padding", "bad"])
+def test_embedding_gradient_of_a_frequent_token(voc, ops, n, V, which):
+    """Positions at even distances hold one token (so do all, a first part of them, no others, or only others do), or one that is left out."""
+    ops.read_status()
+    t = torch.randint(0, V, (n,), device="cuda")
+    there = torch.arange(32, device="cuda") * n // 32
+    token = {"padding": 0, "bad": V + 3}.get(which, V - 1)
+    if which == "first":
+        t[: n // 3] = token
+    elif which == "only there":
+        t[there] = token
+    elif which == "nowhere else":
+        other = t[there]
+        t[:] = token
+        t[there] = other
+    else:
+        t[torch.rand(n, device="cuda") < 0.6] = token
+        t[there] = token
+    _check_grad(voc, torch.randn((n, 4), device="cuda"), t, V, 1.0, 0 if which == "padding" else None)
+    assert ops.read_status() == (4 if which == "bad" else 0)
+
+
+@gpu
 def test_embedding_gradient_through_autograd_and_of_broadcast_gradients(voc):
     w = torch.randn((300, 48), device="cuda").half().requires_grad_(True)
     t = torch.randint(0, 300, (4, 50), device="cuda")
