@@ -68,7 +68,6 @@ constexpr int kFrequent = 8;          // of 32 positions that a frequent token h
 constexpr int kManyTiles = 4;         // from here on a frequent token is looked for
 constexpr int kBatch = 4;             // entries of a lane in flight
 constexpr int kAhead = 7;             // rows that a warp has in flight
-constexpr int kShare = 8;             // entries of a warp's share are a multiple of it
 
 // Rows of the table set to zero by the blocks behind the sorting ones, which wait for their loads most of the time.
 __device__ void zero_table(char *dw, int64_t rows, int64_t row_bytes, int64_t stride_bytes, int64_t block, int64_t blocks) {
@@ -728,10 +727,14 @@ int widest(uintptr_t bits, int size) {  // bytes of the widest vector that addre
     return size;
 }
 
-// Entries of a warp: eight, more where that made over 2 048 pieces.
+// Entries of a warp: the more of a short list's blocks there are, the more SMs add to the table; fewer and longer pieces leave less
+// to join.  Added onto 512 float32 columns with 2, 4, 8 and 16 entries: 1 500 tokens 14.0, 15.9, 18.2 us, 5 000 15.4, 16.5, 20.3, 27.0,
+// 10 000 19.9, 18.1, 20.8, 27.0, 20 000 29.6, 23.5, 22.2, 28.7, 60 000 56.3, 56.3, 47.8, 43.5.  More where that made over 2 048 pieces.
 int warp_entries(int64_t n) {
+    int share = 2;
+    while (share < 16 && share * 4096 < n) share *= 2;
     const int64_t even = (n + 2048 * kSumWarps - 1) / (2048 * kSumWarps);
-    return (int)(even < kShare ? kShare : (even + kShare - 1) / kShare * kShare);
+    return even <= share ? share : (int)((even + 7) / 8 * 8);
 }
 int64_t piece_count(int64_t n) {
     const int64_t length = (int64_t)warp_entries(n) * kSumWarps;
@@ -798,8 +801,8 @@ int launch_embed_backward(const void *grad, int dtype, int64_t g_stride, const i
     const auto bits = [&](const void *a, int64_t stride, int64_t size) {  // of a matrix with H numbers of that size in a row
         return reinterpret_cast<uintptr_t>(a) | (uintptr_t)(stride * size) | (uintptr_t)(H * size);
     };
-    // Up to 256 positions one launch.  Added onto a float32 table of 512 columns: 20, 140 and 256 positions 4.1, 5.3 and 7.5 us (11.7
-    // where one token fills 70 % of 256), by the sorted list 12.0, 13.1 and 13.1 (14.2).
+    // Up to 256 positions one launch.  Added onto a float32 table of 512 columns: 20, 140 and 256 positions 3.2, 5.5 and 6.6 us (11.7
+    // where one token fills 70 % of 256); 257 by the sorted list 11.6 (12.7).
     if (n <= kFew)
         return with_dtype(dtype, [&](auto g) {
             using G = decltype(g);
