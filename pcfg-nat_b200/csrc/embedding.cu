@@ -577,18 +577,18 @@ __global__ void __launch_bounds__(32 * kSumWarps)
 constexpr int kJoinGroups = 16, kJoinColumns = 128;
 
 // The runs that cross pieces: the first part and those of the pieces behind it, sixteen warps taking every sixteenth piece, a
-// lane four columns.
+// lane four columns.  Most blocks only find that no run begins in theirs, so they load all that tells it at once.  With eight warps
+// 28 980 tokens, half of them one, take 26.1 us in all instead of 23.9; with a warp per piece 23.9, but 32 768 of 301 columns 49.4, not 45.3.
 template <typename W>
 __global__ void __launch_bounds__(32 * kJoinGroups)
     embed_join_kernel(int H, Pieces p, W *dw, int64_t dw_stride, float scale, int accumulate) {
     __shared__ float sums[kJoinGroups][kJoinColumns];
     chain_begin();
-    const int total = *p.sorted.total, length = p.length * kSumWarps;
-    const int64_t begin64 = (int64_t)blockIdx.x * length;
-    if (begin64 + length >= total) return;
-    const int begin = (int)begin64, end = begin + length;
+    if (blockIdx.x + 1 == gridDim.x) return;  // nothing behind the last piece
+    const int length = p.length * kSumWarps, begin = blockIdx.x * length, end = begin + length;
+    const int total = *p.sorted.total;
     const int token = p.sorted.token[end - 1], behind = p.sorted.token[end], before = begin > 0 ? p.sorted.token[begin - 1] : -1;
-    if (behind != token || before == token) return;
+    if (end >= total || behind != token || before == token) return;
     const int last = (p.sorted.row_end[token] - 1) / length;  // the piece in which the run ends
     const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, tile = blockIdx.y * kJoinColumns;
     float acc[4] = {};
