@@ -372,9 +372,9 @@ def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
     if len(index) != 1 or min(index) < 0:
         raise RuntimeError("the gradients and outputs must be CUDA tensors on one device")
     kind = [t.dtype for t in every]
-    if not _DTYPES.keys() >= set(kind):
+    types, out_types = set(kind[:n]), set(kind[-n:])
+    if not _DTYPES.keys() >= types | out_types:
         raise RuntimeError("gradients and outputs must be float32, float16 or bfloat16")
-    kind = [_DTYPES[t] for t in kind] if len(set(kind)) > 1 else [_DTYPES[kind[0]]] * len(kind)
     if not all(map(torch.Tensor.is_contiguous, every)):
         for g, o in zip(grads, outs):
             if not _dense(g):
@@ -382,14 +382,15 @@ def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
             if o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
                 raise RuntimeError("an output must have its gradient's layout")
     host = lambda code, v: array.array(code, v)  # read before the call returns
-    src, src_kind, numel = host("Q", at[:n]), host("i", kind[:n]), host("q", size[:n])
+    kinds = lambda k, of: host("i", [_DTYPES[k[0]]]) * n if len(of) == 1 else host("i", map(_DTYPES.__getitem__, k))
+    src, src_kind, numel = host("Q", at[:n]), kinds(kind[:n], types), host("q", size[:n])
     dst, dst_kind = src, src_kind
     if out is not None:
         if size[:n] != size[n:]:
             raise RuntimeError("an output must have its gradient's shape")
-        if any(k and k != j for j, k in zip(kind[:n], kind[n:])):
+        if out_types != {torch.float32} and any(k != j and k != torch.float32 for j, k in zip(kind[:n], kind[n:])):
             raise RuntimeError("an output must be of its gradient's type or float32")
-        dst, dst_kind = host("Q", at[n:]), host("i", kind[n:])
+        dst, dst_kind = host("Q", at[n:]), kinds(kind[n:], out_types)
     dev = grads[0].device
     lib = _cabi.lib()
     head = lambda a: a.buffer_info()[0]

@@ -454,7 +454,7 @@ def test_embedding_gradient_around_the_kernels_limits(voc, n):
 
 
 @gpu
-@pytest.mark.parametrize("n", [257, 5000, 600_000])
+@pytest.mark.parametrize("n", [257, 5000, 600_000, 1_200_000])
 @pytest.mark.parametrize("V", [1, 130, 150_000])
 @pytest.mark.parametrize("which", ["evenly", "first", "only there", "nowhere else", "padding", "bad"])
 def test_embedding_gradient_of_a_frequent_token(voc, ops, n, V, which):
