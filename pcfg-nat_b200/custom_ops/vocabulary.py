@@ -333,12 +333,23 @@ def _dense(t):
     return True
 
 
+def _check_layouts(grads, outs):
+    """Refuses pairs of which the n-th number in memory is not the n-th number of both."""
+    for g, o in zip(grads, outs):
+        if not _dense(g):
+            raise RuntimeError("a gradient must be dense: call contiguous() first")
+        # equal strides alone do not make the output dense: its shape may be another
+        if not (o.is_contiguous() and g.is_contiguous()) and (o.stride() != g.stride() or o.shape != g.shape):
+            raise RuntimeError("an output must have its gradient's layout: both contiguous, or of one shape and the same strides")
+
+
 def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
     """Clips gradients by their global norm, as the trainer does between the backward pass and the optimizer.
 
     norm = ``grad_scale`` * sqrt(sum of all squares); every gradient is multiplied by grad_scale * min(1, max_norm / (norm +
     1e-6)), in place, or into the tensors ``out`` of as many numbers each (of its gradient's type or float32: half-precision
-    gradients into float32 master gradients, with ``grad_scale`` = 1 / loss scale).  ``grads``: a tensor or an iterable of
+    gradients into float32 master gradients, with ``grad_scale`` = 1 / loss scale; contiguous as their gradients, or of the same
+    shape and strides).  ``grads``: a tensor or an iterable of
     tensors of one device, float32, float16 or bfloat16 mixed, any number of them, in any dense layout; None among them is skipped
     (with its output).  Returns the norm before clipping, a float32 tensor on the device; nothing is read back.
 
@@ -376,11 +387,7 @@ def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
     if not _DTYPES.keys() >= types | out_types:
         raise RuntimeError("gradients and outputs must be float32, float16 or bfloat16")
     if not all(map(torch.Tensor.is_contiguous, every)):
-        for g, o in zip(grads, outs):
-            if not _dense(g):
-                raise RuntimeError("a gradient must be dense: call contiguous() first")
-            if o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
-                raise RuntimeError("an output must have its gradient's layout")
+        _check_layouts(grads, outs)
     host = lambda code, v: array.array(code, v)  # read before the call returns
     kinds = lambda k, of: host("i", [_DTYPES[k[0]]]) * n if len(of) == 1 else host("i", map(_DTYPES.__getitem__, k))
     src, src_kind, numel = host("Q", at[:n]), kinds(kind[:n], types), host("q", size[:n])

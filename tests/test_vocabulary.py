@@ -895,3 +895,37 @@ def test_refusals(voc):
     for call, match in cases:
         with pytest.raises(RuntimeError, match=match):
             call()
+
+
+def _pairs_of_equal_strides():
+    """Gradients and outputs of equal strides and as many numbers, but of other shapes: the outputs have gaps."""
+    make = lambda device: [
+        (torch.zeros((4, 3, 2), device=device).permute(2, 1, 0), torch.full((6, 3, 2), 7.0, device=device)[:, :2].permute(2, 1, 0)),
+        (torch.zeros((2, 3), device=device).t(), torch.full((3, 3), 7.0, device=device)[:, :2].t())]
+    return make
+
+
+def test_clipping_asks_for_outputs_of_one_layout(voc):
+    for g, o in _pairs_of_equal_strides()("cpu"):
+        assert g.stride() == o.stride() and g.numel() == o.numel() and voc._dense(g) and not voc._dense(o)
+        with pytest.raises(RuntimeError, match="layout"):
+            voc._check_layouts([g], [o])
+        voc._check_layouts([g], [torch.empty_like(g)])
+        voc._check_layouts([g], [g])
+    flat, one = torch.zeros(12), torch.zeros(3, 4)
+    voc._check_layouts([flat], [one])  # contiguous ones may be of another shape
+    for g, o in ((one.t(), flat), (flat, one.t()), (one.t(), torch.zeros(4, 3))):
+        with pytest.raises(RuntimeError, match="layout"):
+            voc._check_layouts([g], [o])
+    with pytest.raises(RuntimeError, match="dense"):
+        voc._check_layouts([one[:, ::2]], [one[:, ::2]])
+
+
+@gpu
+def test_clipping_leaves_gaps_of_refused_outputs_alone(voc):
+    for g, o in _pairs_of_equal_strides()("cuda"):
+        with pytest.raises(RuntimeError, match="layout"):
+            voc.clip_grad_norm_([g], 1.0, out=[o])
+        assert bool((o._base == 7).all())
+    g = torch.randn((2, 3), device="cuda").t()
+    _check_clip(voc, [g], 0.5, out=[torch.empty_like(g)])
