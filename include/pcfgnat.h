@@ -427,6 +427,10 @@ int pcfgnat_stage_inputs(const void *hidden_src, void *hidden_dst, int row_bytes
 /* ---- The vocabulary table at both ends, and the step behind the backward pass.  No counterpart among the reference's
  * operators: its model looks tokens up with torch's embedding and its trainer clips with torch's operators. ---- */
 
+/* The most tokens, and rows of the table, that the embedding's gradient takes (2^31 - 2^20): what a kernel adds to an index
+ * before it compares it with the end still fits 32 bits.  More are refused (PCFGNAT_ERR_TOO_LARGE). */
+#define PCFGNAT_MAX_INDEX 2146435072
+
 /* Log probabilities of given tokens from materialised logits, with entropy and best alternatives.
  * Row r of the logits (PCFGNAT_DTYPE_*, V numbers in a row) begins (r / rows_inner) * stride_outer + (r % rows_inner) *
  * stride_inner numbers behind `logits`.  tokens [rows]; logprob [rows]; optional (NULL: not wanted) entropy [rows] in nats;
@@ -460,7 +464,7 @@ int pcfgnat_embed(const void *weight, int dtype, int64_t weight_stride, int64_t 
  * whose token is v, in float32 and in an order that the tokens alone decide.  Tokens equal to padding_idx (with has_padding) and
  * tokens out of range (flagged) count for nothing.  d_dtype is PCFGNAT_DTYPE_F32 or grad_out's dtype.  accumulate: added onto the
  * rows that occur, the others stay as they are; otherwise every row is written.  Positions that count for nothing are not read
- * in grad_out.  n, V < 2^31, H <= 2^20.  A few positions need no workspace: 0 bytes, which may be NULL. */
+ * in grad_out.  n, V <= PCFGNAT_MAX_INDEX, H <= 2^20.  A few positions need no workspace: 0 bytes, which may be NULL. */
 size_t pcfgnat_embed_backward_workspace_bytes(int64_t n, int64_t V, int H);
 int pcfgnat_embed_backward(const void *grad_out, int dtype, int64_t grad_stride, const int64_t *tokens, int64_t n, int64_t V,
                            int H, float scale, int has_padding, int64_t padding_idx, void *d_weight, int d_dtype,

@@ -726,7 +726,7 @@ int pcfgnat_embed_backward(const void *grad_out, int dtype, int64_t grad_stride,
     if (n < 0 || V < 1 || H < 1 || grad_stride < 0 || d_stride < H) return PCFGNAT_ERR_INVALID_ARGUMENT;
     if (!d_weight || (n && (!grad_out || !tokens))) return PCFGNAT_ERR_INVALID_ARGUMENT;
     if (dtype < 0 || dtype > PCFGNAT_DTYPE_BF16 || (d_dtype != PCFGNAT_DTYPE_F32 && d_dtype != dtype)) return PCFGNAT_ERR_UNSUPPORTED;
-    if (n > INT32_MAX || V > INT32_MAX || H > (1 << 20)) return PCFGNAT_ERR_TOO_LARGE;
+    if (n > PCFGNAT_MAX_INDEX || V > PCFGNAT_MAX_INDEX || H > (1 << 20)) return PCFGNAT_ERR_TOO_LARGE;
     const size_t need = embed_workspace_bytes(n, V, H);
     if (workspace_bytes < need || (need && !workspace)) return PCFGNAT_ERR_WORKSPACE;
     return launch_embed_backward(grad_out, dtype, grad_stride, tokens, n, V, H, scale, has_padding != 0, padding_idx, d_weight, d_dtype,

@@ -727,7 +727,8 @@ int widest(uintptr_t bits, int size) {  // bytes of the widest vector that addre
     return size;
 }
 
-// Entries of a warp: the more of a short list's blocks there are, the more SMs add to the table; fewer and longer pieces leave less
+// Entries of a warp, for at most PCFGNAT_MAX_INDEX positions 131 008: a share's begin and its length, and the rows staged ahead, add up
+// to less than 2^31.  The more of a short list's blocks there are, the more SMs add to the table; fewer and longer pieces leave less
 // to join.  Added onto 512 float32 columns with 2, 4, 8 and 16 entries: 1 500 tokens 14.0, 15.9, 18.2 us, 5 000 15.4, 16.5, 20.3, 27.0,
 // 10 000 19.9, 18.1, 20.8, 27.0, 20 000 29.6, 23.5, 22.2, 28.7, 60 000 56.3, 56.3, 47.8, 43.5.  More where that made over 2 048 pieces.
 int warp_entries(int64_t n) {

@@ -24,6 +24,7 @@ from .. import _cabi
 from . import pcfg_loss as _ops
 
 MAX_TOP = 32  # PCFGNAT_MAX_TOP
+MAX_INDEX = 2_146_435_072  # PCFGNAT_MAX_INDEX
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # PCFGNAT_DTYPE_*
 
 def _first_derivative(backward):
@@ -221,8 +222,8 @@ def _table(weight, name):
     """(PCFGNAT_DTYPE_*, V, H, numbers between rows) of a table."""
     dt = _numbers(weight, name)
     shape = weight.shape
-    if len(shape) != 2 or not 1 <= shape[0] < 1 << 31 or not 1 <= shape[1] <= 1 << 20:
-        raise RuntimeError(f"{name} must be [V, H] with 1 <= V < 2^31 and 1 <= H <= 2^20")
+    if len(shape) != 2 or not 1 <= shape[0] <= MAX_INDEX or not 1 <= shape[1] <= 1 << 20:
+        raise RuntimeError(f"{name} must be [V, H] with 1 <= V <= {MAX_INDEX} and 1 <= H <= 2^20")
     V, H = shape
     apart, beside = weight.stride()
     if H > 1 and beside != 1 or V > 1 and apart < H:

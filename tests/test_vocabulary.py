@@ -929,3 +929,22 @@ def test_clipping_leaves_gaps_of_refused_outputs_alone(voc):
         assert bool((o._base == 7).all())
     g = torch.randn((2, 3), device="cuda").t()
     _check_clip(voc, [g], 0.5, out=[torch.empty_like(g)])
+
+
+def test_library_refuses_tables_and_lists_whose_indices_could_leave_32_bits(lib, voc):
+    limit, at, room = voc.MAX_INDEX, 16, 1 << 62
+    e = lambda n=1, V=4: lib.pcfgnat_embed_backward(at, 1, 4, at, n, V, 4, 1.0, 0, 0, at, 0, 4, 0, at, room, None, None)
+    for beyond in (limit + 1, (1 << 31) - 130, (1 << 31) - 1, 1 << 31):
+        assert e(n=beyond) == e(V=beyond) == -5
+    # at the limit: the last warp's share of the sorted list, and what a lane looks ahead
+    share = -(-(-(-limit // (2048 * 8))) // 8) * 8
+    begin = (limit - 1) // share * share
+    assert begin + share + 64 < 1 << 31 and limit + 127 < 1 << 31
+
+
+def test_tables_beyond_the_limit_are_refused_by_shape(voc, monkeypatch):
+    monkeypatch.setattr(voc, "_numbers", lambda t, name: 1)  # a tensor without memory stands in for the table
+    for V in (voc.MAX_INDEX + 1, (1 << 31) - 1):
+        with pytest.raises(RuntimeError, match="must be"):
+            voc._table(torch.empty((V, 2), device="meta"), "weight")
+    assert voc._table(torch.empty((voc.MAX_INDEX, 2), device="meta"), "weight") == (1, voc.MAX_INDEX, 2, 2)
