@@ -427,13 +427,13 @@ int pcfgnat_stage_inputs(const void *hidden_src, void *hidden_dst, int row_bytes
 /* ---- The vocabulary table at both ends, and the step behind the backward pass.  No counterpart among the reference's
  * operators: its model looks tokens up with torch's embedding and its trainer clips with torch's operators. ---- */
 
-/* The most tokens, and rows of the table, that the embedding's gradient takes (2^31 - 2^20): what a kernel adds to an index
- * before it compares it with the end still fits 32 bits.  More are refused (PCFGNAT_ERR_TOO_LARGE). */
+/* The longest row of logits, and the most tokens and rows of the table that the embedding's gradient takes (2^31 - 2^20): what a
+ * kernel adds to an index before it compares it with the end still fits 32 bits.  More are refused (PCFGNAT_ERR_TOO_LARGE). */
 #define PCFGNAT_MAX_INDEX 2146435072
 
 /* Log probabilities of given tokens from materialised logits, with entropy and best alternatives.
  * Row r of the logits (PCFGNAT_DTYPE_*, V numbers in a row) begins (r / rows_inner) * stride_outer + (r % rows_inner) *
- * stride_inner numbers behind `logits`.  tokens [rows]; logprob [rows]; optional (NULL: not wanted) entropy [rows] in nats;
+ * stride_inner numbers behind `logits`.  V <= PCFGNAT_MAX_INDEX.  tokens [rows]; logprob [rows]; optional (NULL: not wanted) entropy [rows] in nats;
  * top_logprob and top_index [rows][top] (0 <= top <= PCFGNAT_MAX_TOP), values falling, equal ones by rising index; kept
  * [rows][2] for the backward call.  Everything is formed in float32.
  * Rows whose token is ignore_index (with has_ignore) are left out: 0, 0, (0, -1).  Entries of -inf have no probability and

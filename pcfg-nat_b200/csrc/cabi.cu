@@ -685,7 +685,7 @@ int pcfgnat_token_logprobs(const void *logits, int dtype, int64_t rows, int64_t 
     PCFGNAT_API_RANGE();
     if (rows < 0 || rows_inner < 1 || V < 1 || top < 0 || top > PCFGNAT_MAX_TOP) return PCFGNAT_ERR_INVALID_ARGUMENT;
     if (rows && (!logits || !tokens || !logprob || (top && (!top_logprob || !top_index)))) return PCFGNAT_ERR_INVALID_ARGUMENT;
-    if (rows > INT32_MAX) return PCFGNAT_ERR_TOO_LARGE;
+    if (rows > INT32_MAX || V > PCFGNAT_MAX_INDEX) return PCFGNAT_ERR_TOO_LARGE;
     return launch_token_logprobs(logits, dtype, rows, rows_inner, stride_outer, stride_inner, V, tokens, has_ignore != 0, ignore_index,
                                  top, logprob, entropy, top_logprob, top_index, kept, status, static_cast<cudaStream_t>(stream));
 }
@@ -699,7 +699,7 @@ int pcfgnat_token_logprobs_backward(const void *logits, int dtype, int64_t rows,
     if (rows < 0 || rows_inner < 1 || V < 1 || top < 0 || top > PCFGNAT_MAX_TOP || pitch < V) return PCFGNAT_ERR_INVALID_ARGUMENT;
     if (rows && (!logits || !tokens || !kept || !d_logits || (grad_entropy && !entropy) || (grad_top && top && !top_index)))
         return PCFGNAT_ERR_INVALID_ARGUMENT;
-    if (rows > INT32_MAX) return PCFGNAT_ERR_TOO_LARGE;
+    if (rows > INT32_MAX || V > PCFGNAT_MAX_INDEX) return PCFGNAT_ERR_TOO_LARGE;
     return launch_token_logprobs_grad(logits, dtype, rows, rows_inner, stride_outer, stride_inner, V, tokens, has_ignore != 0,
                                       ignore_index, top, kept, entropy, top_index, grad_logprob, grad_entropy, grad_top, d_logits,
                                       pitch, status, static_cast<cudaStream_t>(stream));

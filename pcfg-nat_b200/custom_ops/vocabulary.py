@@ -127,8 +127,8 @@ def _rows(t):
 
 
 def _logits_rows(logits):
-    if logits.dim() < 1 or not 1 <= logits.shape[-1] < 1 << 31:
-        raise RuntimeError("logits must be [..., V] with V >= 1, below 2^31")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_INDEX:
+        raise RuntimeError(f"logits must be [..., V] with V >= 1, at most {MAX_INDEX}")
     if logits.is_contiguous():
         return logits.numel() // logits.shape[-1] or 1, 0, logits.shape[-1]
     if logits.shape[-1] > 1 and logits.stride(-1) != 1:

@@ -948,3 +948,13 @@ def test_tables_beyond_the_limit_are_refused_by_shape(voc, monkeypatch):
         with pytest.raises(RuntimeError, match="must be"):
             voc._table(torch.empty((V, 2), device="meta"), "weight")
     assert voc._table(torch.empty((voc.MAX_INDEX, 2), device="meta"), "weight") == (1, voc.MAX_INDEX, 2, 2)
+
+
+def test_rows_of_logits_whose_indices_could_leave_32_bits_are_refused(lib, voc):
+    limit, at = voc.MAX_INDEX, 16
+    for V in (limit + 1, (1 << 31) - 511, (1 << 31) - 1):  # the gradient's strided loop steps up to 512 beyond the row
+        assert lib.pcfgnat_token_logprobs(at, 1, 1, 1, 0, V, V, at, 0, 0, 0, at, None, None, None, None, None, None) == -5
+        assert lib.pcfgnat_token_logprobs_backward(at, 1, 1, 1, 0, V, V, at, 0, 0, 0, at, None, None, at, None, None, at, V, None, None) == -5
+        with pytest.raises(RuntimeError, match="V >= 1, at most"):
+            voc._logits_rows(torch.empty((1, V), device="meta"))
+    assert voc._logits_rows(torch.empty((2, limit), device="meta")) == (2, 0, limit) and limit + 4 * 512 < 1 << 31
