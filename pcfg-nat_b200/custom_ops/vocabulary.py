@@ -231,6 +231,14 @@ def _table(weight, name):
     return dt, V, H, max(apart, H)
 
 
+def _padding(padding_idx, rows):
+    """``_optional_index`` of a padding token of a table of that many rows: a negative one counts from the table's end."""
+    there, i = _optional_index(padding_idx, "padding_idx")
+    if there and not -rows <= i < rows:
+        raise RuntimeError(f"padding_idx must be between {-rows} and {rows - 1}, got {i}")
+    return there, i + rows if i < 0 else i
+
+
 def _finite(x, name):
     x = float(x)
     if not math.isfinite(x):
@@ -291,10 +299,10 @@ class EmbedTokensFunc(Function):
 def embed_tokens(weight, tokens, scale=1.0, padding_idx=None):
     """``scale`` * weight[tokens]: [..., H] in the type of ``weight`` [V, H] (float32, float16 or bfloat16; formed in float32,
     rounded once) for ``tokens`` [...] int64.  Differentiable with respect to the table: its gradient is dense, summed in
-    float32 by sorted tokens, the same for the same input; ``padding_idx`` has none, as with torch's embedding.  A token outside
+    float32 by sorted tokens, the same for the same input; ``padding_idx`` has none, as with torch's embedding (-1: the table's last row).  A token outside
     the table: a row of NaN and ``PCFGNAT_STATUS_BAD_INDEX`` in ``read_status``, no gradient."""
     scale = _finite(scale, "scale")
-    padding = _optional_index(padding_idx, "padding_idx")
+    padding = _padding(padding_idx, weight.shape[0]) if isinstance(weight, torch.Tensor) and weight.dim() == 2 else None  # others are refused
     if isinstance(weight, torch.Tensor) and weight.requires_grad and torch.is_grad_enabled():
         return EmbedTokensFunc.apply(weight, tokens, scale, padding)
     return _embed(weight, tokens, scale)
@@ -308,7 +316,7 @@ def embed_tokens_backward(grad_out, tokens, grad_weight, scale=1.0, padding_idx=
     _numbers(grad_out, "grad_out")
     table = _table(grad_weight, "grad_weight")
     scale = _finite(scale, "scale")
-    padding = _optional_index(padding_idx, "padding_idx")
+    padding = _padding(padding_idx, table[1])
     dev = grad_out.device
     if grad_weight.device != dev or grad_weight.dtype not in (torch.float32, grad_out.dtype):
         raise RuntimeError("grad_weight must be float32 or of grad_out's type, on its device")

@@ -958,3 +958,31 @@ def test_rows_of_logits_whose_indices_could_leave_32_bits_are_refused(lib, voc):
         with pytest.raises(RuntimeError, match="V >= 1, at most"):
             voc._logits_rows(torch.empty((1, V), device="meta"))
     assert voc._logits_rows(torch.empty((2, limit), device="meta")) == (2, 0, limit) and limit + 4 * 512 < 1 << 31
+
+
+def test_padding_outside_the_table_is_refused(voc):
+    w, t = torch.zeros((4, 3)), torch.zeros(4, dtype=torch.int64)
+    for bad in (4, -5, 1 << 40):
+        with pytest.raises(RuntimeError, match="padding_idx must be between -4 and 3"):
+            voc.embed_tokens(w, t, padding_idx=bad)
+    assert voc._padding(None, 4) == (0, 0) and voc._padding(-4, 4) == (1, 0) and voc._padding(-1, 4) == (1, 3) and voc._padding(3, 4) == (1, 3)
+
+
+@gpu
+@pytest.mark.parametrize("n", [50, 700])
+@pytest.mark.parametrize("padding", [None, 0, 5, -1, -6])
+def test_padding_counts_from_the_end_as_torchs_does(voc, ops, n, padding):
+    ops.read_status()
+    w = torch.randn((6, 4), device="cuda", requires_grad=True)
+    t = torch.randint(0, 6, (n,), device="cuda")
+    g = torch.randn((n, 4), device="cuda")
+    want, = torch.autograd.grad(torch.nn.functional.embedding(t, w.double(), padding_idx=padding), w, g.double())
+    index = padding if padding is None or padding >= 0 else padding + 6
+    _, room = _grad64(g, t, 6, 1.0, index)
+    d, = torch.autograd.grad(voc.embed_tokens(w, t, padding_idx=padding), w, g)
+    _close(d, want.double(), room + U * want.double().abs())  # torch's is rounded once as it leaves 64 bits
+    direct = voc.embed_tokens_backward(g, t, torch.empty_like(w).detach(), padding_idx=padding, accumulate=False)
+    assert torch.equal(direct, d) and ops.read_status() == 0
+    for bad in (6, -7):
+        with pytest.raises(RuntimeError, match="padding_idx must be between"):
+            voc.embed_tokens_backward(g, t, torch.zeros((6, 4), device="cuda"), padding_idx=bad)
