@@ -25,6 +25,7 @@ from . import pcfg_loss as _ops
 
 MAX_TOP = 32  # PCFGNAT_MAX_TOP
 MAX_INDEX = 2_146_435_072  # PCFGNAT_MAX_INDEX
+_FLOAT_END = 2.0 ** 128 - 2.0 ** 103  # from here on a number rounds to infinity in float32, which the kernels get
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # PCFGNAT_DTYPE_*
 
 def _first_derivative(backward):
@@ -241,8 +242,8 @@ def _padding(padding_idx, rows):
 
 def _finite(x, name):
     x = float(x)
-    if not math.isfinite(x):
-        raise RuntimeError(f"{name} must be finite, got {x}")
+    if not -_FLOAT_END < x < _FLOAT_END:
+        raise RuntimeError(f"{name} must be finite in float32, got {x}")
     return x
 
 

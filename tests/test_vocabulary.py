@@ -986,3 +986,27 @@ def test_padding_counts_from_the_end_as_torchs_does(voc, ops, n, padding):
     for bad in (6, -7):
         with pytest.raises(RuntimeError, match="padding_idx must be between"):
             voc.embed_tokens_backward(g, t, torch.zeros((6, 4), device="cuda"), padding_idx=bad)
+
+
+def test_factors_beyond_float32_are_refused(voc):
+    w, t = torch.zeros((4, 3)), torch.zeros(4, dtype=torch.int64)
+    for bad in (1e39, -1e39, 3.5e38):
+        with pytest.raises(RuntimeError, match="scale must be finite"):
+            voc.embed_tokens(w, t, scale=bad)
+        with pytest.raises(RuntimeError, match="grad_scale must be finite"):
+            voc._finite(bad, "grad_scale")
+    last = math.nextafter(2.0 ** 128 - 2.0 ** 103, 0)
+    assert math.isfinite(ctypes.c_float(last).value) and math.isinf(ctypes.c_float(2.0 ** 128 - 2.0 ** 103).value)
+    assert voc._finite(last, "scale") == last and voc._finite(1, "scale") == 1.0 and voc._finite(1e-50, "scale") == 1e-50
+
+
+@gpu
+def test_factors_beyond_float32_are_refused_by_every_operator(voc):
+    w, t = torch.ones((4, 3), device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    for bad in (1e39, -math.inf, math.nan):
+        for call in (lambda: voc.embed_tokens(w, t, scale=bad), lambda: voc.clip_grad_norm_(w, 1.0, grad_scale=bad),
+                     lambda: voc.embed_tokens_backward(torch.ones((4, 3), device="cuda"), t, w, scale=bad)):
+            with pytest.raises(RuntimeError, match="scale must be finite"):
+                call()
+    assert bool((w == 1).all())
+    assert torch.equal(voc.embed_tokens(w, t, scale=3e38), w * 3e38)
