@@ -369,6 +369,8 @@ def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise RuntimeError(f"max_norm must be 0 or more, got {max_norm}")
+    if _FLOAT_END <= max_norm < math.inf:  # a limit all the same, where infinity is none
+        max_norm = torch.finfo(torch.float32).max
     grad_scale = _finite(grad_scale, "grad_scale")
     listed = lambda g: [g] if isinstance(g, torch.Tensor) else list(g)
     grads = listed(grads)

@@ -1010,3 +1010,15 @@ def test_factors_beyond_float32_are_refused_by_every_operator(voc):
                 call()
     assert bool((w == 1).all())
     assert torch.equal(voc.embed_tokens(w, t, scale=3e38), w * 3e38)
+
+
+@gpu
+@pytest.mark.parametrize("limit", [3e38, 1e39, 1e300])
+def test_a_finite_limit_beyond_float32_is_a_limit(voc, limit):
+    """A norm of NaN makes every gradient NaN and an infinite one makes them 0 whatever the limit is, unless there is none."""
+    g = torch.tensor([1.0, math.nan], device="cuda")
+    assert math.isnan(float(voc.clip_grad_norm_(g, limit))) and bool(g.isnan().all())
+    g = torch.tensor([1.0, math.inf], device="cuda")
+    assert float(voc.clip_grad_norm_(g, limit)) == math.inf and g[0] == 0 and g[1].isnan()
+    g = torch.tensor([3.0, 4.0], device="cuda")
+    assert float(voc.clip_grad_norm_(g, limit)) == 5 and g.tolist() == [3.0, 4.0]
