@@ -1022,3 +1022,30 @@ def test_a_finite_limit_beyond_float32_is_a_limit(voc, limit):
     assert float(voc.clip_grad_norm_(g, limit)) == math.inf and g[0] == 0 and g[1].isnan()
     g = torch.tensor([3.0, 4.0], device="cuda")
     assert float(voc.clip_grad_norm_(g, limit)) == 5 and g.tolist() == [3.0, 4.0]
+
+
+def test_forward_mode_tangents_are_refused(voc, monkeypatch):
+    monkeypatch.setattr(voc._ops, "_require_cuda", lambda: None)
+    w, t = torch.ones((4, 3)), torch.zeros(4, dtype=torch.int64)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: voc.token_logprobs(dual, t), lambda: voc.embed_tokens(dual, t), lambda: voc.embed_tokens_backward(dual, t, w),
+                     lambda: voc.embed_tokens_backward(w, t, dual), lambda: voc.clip_grad_norm_(dual, 1.0),
+                     lambda: voc.clip_grad_norm_([w, None], 1.0, out=[dual, None])):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        voc._no_tangents(w, t, None)  # others go on while a level is open
+    voc._no_tangents(dual)
+
+
+@gpu
+def test_forward_mode_tangents_are_refused_before_anything_is_written(voc):
+    w, t = torch.ones((4, 3), device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(w.clone(), torch.ones_like(w))
+        for call in (lambda: voc.token_logprobs(dual, t, top=1), lambda: voc.embed_tokens(dual, t), lambda: voc.clip_grad_norm_(dual, 1.0),
+                     lambda: voc.embed_tokens_backward(dual, t, w, accumulate=False), lambda: voc.embed_tokens_backward(w, t, dual)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        assert bool((w == 1).all()) and bool((torch.autograd.forward_ad.unpack_dual(dual).primal == 1).all())
+        assert torch.equal(voc.embed_tokens(w, t), w)
