@@ -17,7 +17,7 @@ import math
 from collections import namedtuple
 
 import torch
-from torch.autograd import Function, forward_ad
+from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from .. import _cabi
@@ -52,12 +52,6 @@ def _numbers(t, name):
     if dt is None:
         raise RuntimeError(f"{name} must be float32, float16 or bfloat16 (got {t.dtype})")
     return dt
-
-
-def _no_tangents(*tensors):
-    """Refuses inputs with a forward-mode tangent, which kernels that are given addresses would drop."""
-    if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
-        raise RuntimeError("forward-mode derivatives of this operator are not supported")
 
 
 class _Stay:
@@ -220,7 +214,7 @@ def token_logprobs(logits, tokens, top=0, entropy=False, ignore_index=None):
     if not 0 <= top <= MAX_TOP:
         raise RuntimeError(f"top must be between 0 and {MAX_TOP}, got {top}")
     ignore = _optional_index(ignore_index, "ignore_index")
-    _no_tangents(logits)
+    _ops._no_tangents(logits)
     if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*TokenLogprobsFunc.apply(logits, tokens, top, bool(entropy), ignore))
     return TokenLogprobs(*_token_logprobs(logits, tokens, top, entropy, ignore, False)[:4])
@@ -310,7 +304,7 @@ def embed_tokens(weight, tokens, scale=1.0, padding_idx=None):
     float32 by sorted tokens, the same for the same input; ``padding_idx`` has none, as with torch's embedding (-1: the table's last row).  A token outside
     the table: a row of NaN and ``PCFGNAT_STATUS_BAD_INDEX`` in ``read_status``, no gradient."""
     scale = _finite(scale, "scale")
-    _no_tangents(weight)
+    _ops._no_tangents(weight)
     padding = _padding(padding_idx, weight.shape[0]) if isinstance(weight, torch.Tensor) and weight.dim() == 2 else None  # others are refused
     if isinstance(weight, torch.Tensor) and weight.requires_grad and torch.is_grad_enabled():
         return EmbedTokensFunc.apply(weight, tokens, scale, padding)
@@ -322,7 +316,7 @@ def embed_tokens_backward(grad_out, tokens, grad_weight, scale=1.0, padding_idx=
     shares, whose ``d weight`` (float32 from ``proj_backward_products``, float16 from ``runtime.LossStep(proj_backward=True)``) it
     completes without a second dense tensor.  Rows whose token does not occur are not touched.  ``accumulate=False``: every row is
     overwritten.  ``grad_weight`` is float32 or of ``grad_out``'s type."""
-    _no_tangents(grad_out, grad_weight)
+    _ops._no_tangents(grad_out, grad_weight)
     _numbers(grad_out, "grad_out")
     table = _table(grad_weight, "grad_weight")
     scale = _finite(scale, "scale")
@@ -386,7 +380,7 @@ def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
     outs = grads if out is None else listed(out)
     if len(outs) != len(grads):
         raise RuntimeError("out must hold one tensor per gradient")
-    _no_tangents(*grads, *outs)
+    _ops._no_tangents(*grads, *outs)
     # one plain pass over the list for each question: a model has hundreds of gradients, and the kernels are done with them sooner
     every = grads if out is None else grads + outs
     try:

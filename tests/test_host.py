@@ -252,3 +252,14 @@ def test_kernels_meet_before_they_touch_a_peers_shared_memory():
             assert met and met.start() < min(uses), f"{file}: {name}"
     assert {"lookahead_decode_kernel", "viterbi_cluster_kernel", "inside_cluster_kernel", "inside_exact_kernel",
             "outside_cluster_kernel", "inside_linear_kernel", "outside_linear_kernel", "proj_kernel"} <= seen, seen
+
+
+def test_links_refuse_forward_mode_tangents(ops):
+    """Whether the features need a gradient or not: the kernels get their addresses, not their tangents."""
+    features = [torch.zeros((1, 4, 1, 32)) for _ in range(3)] + [torch.zeros((1, 4, 1))]
+    with torch.autograd.forward_ad.dual_level():
+        for i in range(4):
+            dual = list(features)
+            dual[i] = torch.autograd.forward_ad.make_dual(features[i], torch.ones_like(features[i]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                ops._Kernel.extract_links(*dual, None, 1, None, None, None)
