@@ -64,18 +64,20 @@ __device__ __forceinline__ double block_sum(double v, double *part) {
     return v;
 }
 
-// The squares of a vector's numbers.  Those of half-precision numbers have at most 22 bits: in float32 every product is exact and
-// a sum of eight is rounded seven times; the sum is added in 64 bits.  bfloat16 numbers have the range of float32, so sums that
-// left float32's range, or come near its lower end, are formed again in 64 bits.
+// The squares of a vector's numbers.  Those of half-precision numbers have at most 22 bits: in float32 every product is exact, and
+// the eight are added by pairs, so that each passes three roundings of 2^-24 (one after the other the sum could lose 7 of them); the
+// sum is added in 64 bits.  The norm is then off by at most 1.5 * 2^-24 before its own rounding.  bfloat16 numbers have the range of
+// float32, so sums that left float32's range, or come near its lower end, are formed again in 64 bits.
 template <typename T>
 __device__ __forceinline__ double squares(const uint4 &raw) {
     constexpr int kVec = RowCut<T>::kVec;
     float x[kVec];
     unpack_vec<T, kVec>(raw, x);
     if constexpr (sizeof(T) == 2) {
-        float s = 0.f;
+        float two[kVec / 2];
 #pragma unroll
-        for (int j = 0; j < kVec; j++) s = fmaf(x[j], x[j], s);
+        for (int j = 0; j < kVec / 2; j++) two[j] = fmaf(x[2 * j], x[2 * j], x[2 * j + 1] * x[2 * j + 1]);
+        const float s = (two[0] + two[1]) + (two[2] + two[3]);
         if (std::is_same_v<T, __half> || (s >= 1e-25f && s <= 1e37f)) return s;
         if (((raw.x | raw.y | raw.z | raw.w) & 0x7fff7fffu) == 0) return 0.0;
     }

@@ -1049,3 +1049,16 @@ def test_forward_mode_tangents_are_refused_before_anything_is_written(voc):
                 call()
         assert bool((w == 1).all()) and bool((torch.autograd.forward_ad.unpack_dual(dual).primal == 1).all())
         assert torch.equal(voc.embed_tokens(w, t), w)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_norm_of_halves_keeps_small_numbers_beside_large_ones(voc, dtype):
+    """1 and seven numbers whose squares, 2^-24, are half a step of it: added one after the other they vanish.  In 64 bits the sum of
+    n such vectors is n (1 + 7 u); added by pairs, eight squares are off by three roundings at most, the norm by half of that and one
+    rounding of its own: 2.5 u."""
+    for n in (1, 67, 1059, 3000):
+        g = torch.full((n, 8), 2.0 ** -12, device="cuda", dtype=dtype)
+        g[:, 0] = 1
+        want = math.sqrt(n * (1 + 7 * U))
+        assert abs(float(voc.clip_grad_norm_([g], math.inf)) - want) <= 2.5 * U * (1 + 8 * U) * want
