@@ -44,7 +44,7 @@ def _require_cuda():
         raise RuntimeError("You need GPU to use the custom cuda operations")
 
 
-def _no_tangents(*tensors):
+def _no_tangents(tensors):
     """Refuses inputs with a forward-mode tangent, which kernels that are given addresses would drop."""
     if forward_ad._current_level >= 0 and any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError("forward-mode derivatives of this operator are not supported")
@@ -880,7 +880,7 @@ class _Kernel:
         or 64 per head without score matrices in memory (``pcfgnat_links_fused``); others, and a few long sentences, in
         three launches: feature gather, the per-head score products, and masking + joint log-softmax + head mixture.
         Differentiable with respect to the four feature tensors (``ExtractLinksFunc``)."""
-        _no_tangents(query, key_left, key_right, gate_logits)
+        _no_tangents((query, key_left, key_right, gate_logits))
         if torch.is_grad_enabled() and any(t.requires_grad for t in (query, key_left, key_right, gate_logits)):
             return ExtractLinksFunc.apply(query, key_left, key_right, gate_logits, prev_output_tokens, pad_index,
                                           left_tree_mask, right_tree_mask, main_chain)

@@ -13,6 +13,7 @@ The arguments are checked, outputs allocated with torch, and the kernels run on 
 nothing is copied to the host.  There is no CPU path, and no forward-mode derivative: inputs with a tangent are refused.
 """
 import array
+import itertools
 import math
 from collections import namedtuple
 
@@ -214,7 +215,7 @@ def token_logprobs(logits, tokens, top=0, entropy=False, ignore_index=None):
     if not 0 <= top <= MAX_TOP:
         raise RuntimeError(f"top must be between 0 and {MAX_TOP}, got {top}")
     ignore = _optional_index(ignore_index, "ignore_index")
-    _ops._no_tangents(logits)
+    _ops._no_tangents((logits,))
     if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
         return TokenLogprobs(*TokenLogprobsFunc.apply(logits, tokens, top, bool(entropy), ignore))
     return TokenLogprobs(*_token_logprobs(logits, tokens, top, entropy, ignore, False)[:4])
@@ -304,7 +305,7 @@ def embed_tokens(weight, tokens, scale=1.0, padding_idx=None):
     float32 by sorted tokens, the same for the same input; ``padding_idx`` has none, as with torch's embedding (-1: the table's last row).  A token outside
     the table: a row of NaN and ``PCFGNAT_STATUS_BAD_INDEX`` in ``read_status``, no gradient."""
     scale = _finite(scale, "scale")
-    _ops._no_tangents(weight)
+    _ops._no_tangents((weight,))
     padding = _padding(padding_idx, weight.shape[0]) if isinstance(weight, torch.Tensor) and weight.dim() == 2 else None  # others are refused
     if isinstance(weight, torch.Tensor) and weight.requires_grad and torch.is_grad_enabled():
         return EmbedTokensFunc.apply(weight, tokens, scale, padding)
@@ -316,7 +317,7 @@ def embed_tokens_backward(grad_out, tokens, grad_weight, scale=1.0, padding_idx=
     shares, whose ``d weight`` (float32 from ``proj_backward_products``, float16 from ``runtime.LossStep(proj_backward=True)``) it
     completes without a second dense tensor.  Rows whose token does not occur are not touched.  ``accumulate=False``: every row is
     overwritten.  ``grad_weight`` is float32 or of ``grad_out``'s type."""
-    _ops._no_tangents(grad_out, grad_weight)
+    _ops._no_tangents((grad_out, grad_weight))
     _numbers(grad_out, "grad_out")
     table = _table(grad_weight, "grad_weight")
     scale = _finite(scale, "scale")
@@ -380,7 +381,7 @@ def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
     outs = grads if out is None else listed(out)
     if len(outs) != len(grads):
         raise RuntimeError("out must hold one tensor per gradient")
-    _ops._no_tangents(*grads, *outs)
+    _ops._no_tangents(itertools.chain(grads, outs))
     # one plain pass over the list for each question: a model has hundreds of gradients, and the kernels are done with them sooner
     every = grads if out is None else grads + outs
     try:

@@ -1034,8 +1034,8 @@ def test_forward_mode_tangents_are_refused(voc, monkeypatch):
                      lambda: voc.clip_grad_norm_([w, None], 1.0, out=[dual, None])):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
-        voc._ops._no_tangents(w, t, None)  # others go on while a level is open
-    voc._ops._no_tangents(dual)
+        voc._ops._no_tangents((w, t, None))  # others go on while a level is open
+    voc._ops._no_tangents((dual,))
 
 
 @gpu
