@@ -463,7 +463,8 @@ int pcfgnat_embed(const void *weight, int dtype, int64_t weight_stride, int64_t 
 /* The table's gradient: row v of d_weight [V] (grad_stride, d_stride: numbers between rows) = scale * the sum of grad_out's rows
  * whose token is v, in float32 and in an order that the tokens alone decide.  Tokens equal to padding_idx (with has_padding) and
  * tokens out of range (flagged) count for nothing.  d_dtype is PCFGNAT_DTYPE_F32 or grad_out's dtype.  accumulate: added onto the
- * rows that occur, the others stay as they are; otherwise every row is written.  Positions that count for nothing are not read
+ * rows that occur, the others stay as they are (onto a float32 table numbers and sums below 2^-126 count as 0, as PTX has it for
+ * float32 reductions in global memory); otherwise every row is written.  Positions that count for nothing are not read
  * in grad_out.  n, V <= PCFGNAT_MAX_INDEX, H <= 2^20.  A few positions need no workspace: 0 bytes, which may be NULL. */
 size_t pcfgnat_embed_backward_workspace_bytes(int64_t n, int64_t V, int H);
 int pcfgnat_embed_backward(const void *grad_out, int dtype, int64_t grad_stride, const int64_t *tokens, int64_t n, int64_t V,

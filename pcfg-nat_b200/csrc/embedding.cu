@@ -389,7 +389,9 @@ __global__ void __launch_bounds__(kSortThreads, 1)
 }
 
 // A finished sum into the table.  Every number of the table gets at most one sum per call, so adding to a float32 table by a
-// reduction (which needs not wait for what is there) has one order only.
+// reduction (which needs not wait for what is there) has one order only.  A reduction takes operands and results below the least normal
+// number, 2^-126, for 0.  Reading, adding and writing instead, which keeps them, takes 36.7 us where 28 980 halves of 512 columns take 31.3 by
+// reductions (four tables in turn, so that none is in L2), 68 where 60 000 take 49; with the table's row read ahead 35.5 and 58.
 template <typename T, int VEC>
 __device__ __forceinline__ void write_row(T *p, const float (&acc)[VEC], float scale, int accumulate) {
     if constexpr (sizeof(T) == 4) {

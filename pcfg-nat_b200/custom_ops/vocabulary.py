@@ -315,7 +315,8 @@ def embed_tokens(weight, tokens, scale=1.0, padding_idx=None):
 def embed_tokens_backward(grad_out, tokens, grad_weight, scale=1.0, padding_idx=None, accumulate=True):
     """Adds the gradient of ``embed_tokens`` onto ``grad_weight`` [V, H] and returns it: for a table that the output projection
     shares, whose ``d weight`` (float32 from ``proj_backward_products``, float16 from ``runtime.LossStep(proj_backward=True)``) it
-    completes without a second dense tensor.  Rows whose token does not occur are not touched.  ``accumulate=False``: every row is
+    completes without a second dense tensor.  Rows whose token does not occur are not touched; in the others a float32 number below 2^-126, of the table or
+    the sum, counts as 0.  ``accumulate=False``: every row is
     overwritten.  ``grad_weight`` is float32 or of ``grad_out``'s type."""
     _ops._no_tangents((grad_out, grad_weight))
     _numbers(grad_out, "grad_out")

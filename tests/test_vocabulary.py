@@ -1062,3 +1062,32 @@ def test_the_norm_of_halves_keeps_small_numbers_beside_large_ones(voc, dtype):
         g[:, 0] = 1
         want = math.sqrt(n * (1 + 7 * U))
         assert abs(float(voc.clip_grad_norm_([g], math.inf)) - want) <= 2.5 * U * (1 + 8 * U) * want
+
+
+@gpu
+@pytest.mark.parametrize("H", [7, 8])
+@pytest.mark.parametrize("n", [6, 700])
+@pytest.mark.parametrize("into", TYPES)
+def test_embedding_gradient_beside_numbers_below_the_least_normal_one(voc, into, n, H):
+    """Subnormal numbers of the table and of the gradient: kept in rows that do not occur, in a table that is overwritten, and in tables
+    of halves.  What is added onto a float32 table may take each of the two operands and the result for 0."""
+    least = torch.finfo(into).tiny
+    t = torch.arange(n, device="cuda") % 3
+    g = torch.zeros((n, H), device="cuda", dtype=into)
+    g[0], g[1] = least / 4, least * 8  # token 0 below the least normal number, token 1 above
+    table = torch.full((5, H), least / 2, device="cuda", dtype=into)
+    more = table.clone()
+    voc.embed_tokens_backward(g, t, more)
+    want = table.double()
+    want[0] += least / 4
+    want[1] += least * 8
+    assert torch.equal(more[3:], table[3:])  # no token of theirs: not touched
+    if into == torch.float32:
+        room = torch.full_like(want, 0.75 * least)  # all there is: least / 2 and least / 4, both taken for 0, or their sum
+        room[1] = least / 2  # the table's; the result is a normal number
+        _close(more, want, room)
+    else:
+        assert torch.equal(more.double(), want)
+    d = voc.embed_tokens_backward(g, t, torch.empty_like(table), accumulate=False)
+    want -= table.double()
+    assert torch.equal(d.double(), want)
