@@ -1091,3 +1091,27 @@ def test_embedding_gradient_beside_numbers_below_the_least_normal_one(voc, into,
     d = voc.embed_tokens_backward(g, t, torch.empty_like(table), accumulate=False)
     want -= table.double()
     assert torch.equal(d.double(), want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype, into", [(torch.float32, torch.float32), (torch.float16, torch.float16), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("n", [0, 40, 256, 257, 6000])
+@pytest.mark.parametrize("V", [1, 2, 3, 700, 150_000])
+def test_embedding_gradient_into_columns_of_a_wider_table(voc, dtype, into, n, V):
+    """Rows further apart than they are long, at any place of a 16-byte vector: what lies between them stays as it is."""
+    gen = torch.Generator(device="cuda").manual_seed(V + n)
+    for first, H, wide in ((8, 48, 64), (3, 48, 61), (1, 13, 16), (16, 8, 24), (0, 5, 7)):
+        g = torch.randn((n, H), generator=gen, device="cuda").to(dtype)
+        t = torch.randint(0, V, (n,), generator=gen, device="cuda")
+        t[: n // 2] = V // 2
+        want, room = _grad64(g, t, V, 1.5, 0)
+        table = torch.full((V, wide), 7.0, device="cuda", dtype=into)
+        part = table[:, first:first + H]
+        part.fill_(math.nan)
+        voc.embed_tokens_backward(g, t, part, scale=1.5, padding_idx=0, accumulate=False)
+        _close(part, want, room, into)
+        start = torch.randn((V, H), generator=gen, device="cuda").to(into)
+        part.copy_(start)
+        voc.embed_tokens_backward(g, t, part, scale=1.5, padding_idx=0)
+        _close(part, want + start.double(), room + U * (want.abs() + start.double().abs()), into)
+        assert bool((table[:, :first] == 7).all()) and bool((table[:, first + H:] == 7).all())
