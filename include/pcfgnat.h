@@ -461,7 +461,7 @@ int pcfgnat_token_logprobs_backward(const void *logits, int dtype, int64_t rows,
 int pcfgnat_embed(const void *weight, int dtype, int64_t weight_stride, int64_t V, int H, const int64_t *tokens, int64_t n,
                   float scale, void *out, int *status, void *stream);
 /* The table's gradient: row v of d_weight [V] (grad_stride, d_stride: numbers between rows) = scale * the sum of grad_out's rows
- * whose token is v, in float32 and in an order that the tokens alone decide.  Tokens equal to padding_idx (with has_padding) and
+ * whose token is v, in float32 and in an order that the tokens, the types and (for few positions) the matrices' alignment decide.  Tokens equal to padding_idx (with has_padding) and
  * tokens out of range (flagged) count for nothing.  d_dtype is PCFGNAT_DTYPE_F32 or grad_out's dtype.  accumulate: added onto the
  * rows that occur, the others stay as they are (onto a float32 table numbers and sums below 2^-126 count as 0, as PTX has it for
  * float32 reductions in global memory); otherwise every row is written.  Positions that count for nothing are not read
@@ -476,7 +476,8 @@ int pcfgnat_embed_backward(const void *grad_out, int dtype, int64_t grad_stride,
  * c = min(1, max_norm / (norm + 1e-6))  dst[i] = c * grad_scale * src[i], the products formed in float32.  dst[i] is src[i]
  * itself (left alone where c * grad_scale is 1) or memory that overlaps no other tensor (PCFGNAT_ERR_INVALID_ARGUMENT
  * otherwise); dst_dtype[i] is src_dtype[i] or PCFGNAT_DTYPE_F32.  The arrays are host memory and are read before the call
- * returns; sums are held in float64 and do not depend on timing.  A norm of NaN makes every output NaN; an infinite one makes them
+ * returns; sums are held in float64 (of halves, eight squares are added by pairs in float32 first: the norm is off by at most 2.5 * 2^-24
+ * of itself) in an order that sizes, types, addresses modulo 16 and the number of SMs decide.  A norm of NaN makes every output NaN; an infinite one makes them
  * 0, and NaN where the gradient is infinite or NaN; an infinite max_norm means c = 1 whatever the norm. */
 size_t pcfgnat_clip_grad_norm_workspace_bytes(int n);
 int pcfgnat_clip_grad_norm(int n, const void *const *src, const int *src_dtype, void *const *dst, const int *dst_dtype,

@@ -3,8 +3,8 @@
 // Two launches for up to kMaxTensors tensors, whose addresses and lengths travel as kernel parameters (copied at the launch, so
 // that a captured graph holds them): squares summed per block into the caller's scratch memory, then every block adds up the
 // blocks' sums in the same order, forms the factor, and scales its share.  Nothing is scaled where the factor is 1 and a tensor
-// is its own output.  Squares and sums are held in 64 bits: the square of a float32 gradient beyond 1.8e19 or below 1e-19 has
-// no float32.
+// is its own output.  Sums are held in 64 bits, and so are the squares of float32 gradients: beyond 1.8e19 or below 1e-19 they have
+// no float32.  Of halves, eight squares are added in float32 before.
 #include "row_vectors.cuh"
 
 namespace pcfgnat {

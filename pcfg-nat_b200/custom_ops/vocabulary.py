@@ -11,6 +11,8 @@ know of the row.  ``embed_tokens`` takes what ``glance_select`` gives (the decod
 step of ``runtime.GlanceStep``; its gradient can be added onto the projection's ``d weight`` where the table is shared.
 The arguments are checked, outputs allocated with torch, and the kernels run on the tensors' device and its current stream;
 nothing is copied to the host.  There is no CPU path, and no forward-mode derivative: inputs with a tangent are refused.
+All can be captured into a CUDA graph.  One that is captured before anything of this package ran on its device has no status word:
+what such a graph does with bad tokens is the same, but ``read_status`` does not tell of it.
 """
 import array
 import itertools
@@ -302,7 +304,7 @@ class EmbedTokensFunc(Function):
 def embed_tokens(weight, tokens, scale=1.0, padding_idx=None):
     """``scale`` * weight[tokens]: [..., H] in the type of ``weight`` [V, H] (float32, float16 or bfloat16; formed in float32,
     rounded once) for ``tokens`` [...] int64.  Differentiable with respect to the table: its gradient is dense, summed in
-    float32 by sorted tokens, the same for the same input; ``padding_idx`` has none, as with torch's embedding (-1: the table's last row).  A token outside
+    float32 by sorted tokens, the same for the same input at the same alignment; ``padding_idx`` has none, as with torch's embedding (-1: the table's last row).  A token outside
     the table: a row of NaN and ``PCFGNAT_STATUS_BAD_INDEX`` in ``read_status``, no gradient."""
     scale = _finite(scale, "scale")
     _ops._no_tangents((weight,))
@@ -361,15 +363,16 @@ def _check_layouts(grads, outs):
 def clip_grad_norm_(grads, max_norm, out=None, grad_scale=1.0):
     """Clips gradients by their global norm, as the trainer does between the backward pass and the optimizer.
 
-    norm = ``grad_scale`` * sqrt(sum of all squares); every gradient is multiplied by grad_scale * min(1, max_norm / (norm +
+    norm = abs(``grad_scale``) * sqrt(sum of all squares); every gradient is multiplied by grad_scale * min(1, max_norm / (norm +
     1e-6)), in place, or into the tensors ``out`` of as many numbers each (of its gradient's type or float32: half-precision
     gradients into float32 master gradients, with ``grad_scale`` = 1 / loss scale; contiguous as their gradients, or of the same
     shape and strides).  ``grads``: a tensor or an iterable of
     tensors of one device, float32, float16 or bfloat16 mixed, any number of them, in any dense layout; None among them is skipped
     (with its output).  Returns the norm before clipping, a float32 tensor on the device; nothing is read back.
 
-    ``max_norm=math.inf`` only measures and scales by ``grad_scale``, whatever the norm; 0 makes every gradient 0.  Squares are summed in float64, in an order that the
-    sizes alone decide.  A norm of NaN makes every gradient NaN; an infinite one makes finite gradients 0."""
+    ``max_norm=math.inf`` only measures and scales by ``grad_scale``, whatever the norm; 0 makes every gradient 0.  Squares are
+    summed in float64 (those of half-precision numbers by eights in float32 first), in an order that does not depend on timing:
+    sizes, types, alignment and the number of SMs decide it.  A norm of NaN makes every gradient NaN; an infinite one makes finite gradients 0."""
     _ops._require_cuda()
     max_norm = float(max_norm)
     if not max_norm >= 0:
