@@ -207,7 +207,7 @@ def token_logprobs(logits, tokens, top=0, entropy=False, ignore_index=None):
     ``entropy``: also the row's entropy in nats.  ``top`` (up to 32): also its best alternatives, ``top_logprob`` and
     ``top_index`` [..., top], falling, equal ones by rising index.  What is not asked for is None in the result, a
     ``TokenLogprobs``.  Differentiable with respect to the logits through logprob, entropy and top_logprob; the gradient is
-    formed in float32 and rounded once, and the logits must still hold what the forward saw.
+    formed in float32 (probabilities below 2^-126 count as 0) and rounded once, and the logits must still hold what the forward saw.
 
     Rows whose token is ``ignore_index`` (padding) are not read: logprob, entropy and top_logprob 0, top_index -1, gradient 0.
     -inf masks an entry: it is no alternative, and where fewer than ``top`` are left the rest is (-inf, -1).  A row of nothing
