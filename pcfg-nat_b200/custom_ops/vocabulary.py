@@ -236,9 +236,9 @@ def _table(weight, name):
     return dt, V, H, max(apart, H)
 
 
-def _padding(padding_idx, rows):
-    """``_optional_index`` of a padding token of a table of that many rows: a negative one counts from the table's end."""
-    there, i = _optional_index(padding_idx, "padding_idx")
+def _padding(given, rows):
+    """An ``_optional_index`` as the row of a table of that many: a negative one counts from the table's end."""
+    there, i = given
     if there and not -rows <= i < rows:
         raise RuntimeError(f"padding_idx must be between {-rows} and {rows - 1}, got {i}")
     return there, i + rows if i < 0 else i
@@ -251,8 +251,10 @@ def _finite(x, name):
     return x
 
 
-def _embed(weight, tokens, scale):
+def _embed(weight, tokens, scale, padding):
     dt, V, H, apart = _table(weight, "weight")
+    if not -V <= padding[1] < V:
+        _padding(padding, V)  # nothing to do here, but refused where the gradient would be
     dev = weight.device
     tokens = _token_tensor(tokens, dev)
     with _on(dev):
@@ -286,10 +288,10 @@ def _embed_backward(g, tokens, d_weight, table, scale, padding, accumulate):  # 
 class EmbedTokensFunc(Function):
     @staticmethod
     def forward(ctx, weight, tokens, scale, padding):
-        out = _embed(weight, tokens, scale)  # checks them
+        out = _embed(weight, tokens, scale, padding)  # checks them
         ctx.save_for_backward(tokens.contiguous())
         V, H = ctx.shape = weight.shape
-        ctx.scale, ctx.padding, ctx.table = scale, padding, (_DTYPES[weight.dtype], V, H, H)  # the gradient's, which is contiguous
+        ctx.scale, ctx.padding, ctx.table = scale, _padding(padding, V), (_DTYPES[weight.dtype], V, H, H)  # the gradient's, which is contiguous
         return out
 
     @staticmethod
@@ -307,11 +309,11 @@ def embed_tokens(weight, tokens, scale=1.0, padding_idx=None):
     float32 by sorted tokens, the same for the same input at the same alignment; ``padding_idx`` has none, as with torch's embedding (-1: the table's last row).  A token outside
     the table: a row of NaN and ``PCFGNAT_STATUS_BAD_INDEX`` in ``read_status``, no gradient."""
     scale = _finite(scale, "scale")
+    padding = _optional_index(padding_idx, "padding_idx")
     _ops._no_tangents((weight,))
-    padding = _padding(padding_idx, weight.shape[0]) if isinstance(weight, torch.Tensor) and weight.dim() == 2 else None  # others are refused
     if isinstance(weight, torch.Tensor) and weight.requires_grad and torch.is_grad_enabled():
         return EmbedTokensFunc.apply(weight, tokens, scale, padding)
-    return _embed(weight, tokens, scale)
+    return _embed(weight, tokens, scale, padding)
 
 
 def embed_tokens_backward(grad_out, tokens, grad_weight, scale=1.0, padding_idx=None, accumulate=True):
@@ -324,7 +326,7 @@ def embed_tokens_backward(grad_out, tokens, grad_weight, scale=1.0, padding_idx=
     _numbers(grad_out, "grad_out")
     table = _table(grad_weight, "grad_weight")
     scale = _finite(scale, "scale")
-    padding = _padding(padding_idx, table[1])
+    padding = _padding(_optional_index(padding_idx, "padding_idx"), table[1])
     dev = grad_out.device
     if grad_weight.device != dev or grad_weight.dtype not in (torch.float32, grad_out.dtype):
         raise RuntimeError("grad_weight must be float32 or of grad_out's type, on its device")

@@ -960,12 +960,16 @@ def test_rows_of_logits_whose_indices_could_leave_32_bits_are_refused(lib, voc):
     assert voc._logits_rows(torch.empty((2, limit), device="meta")) == (2, 0, limit) and limit + 4 * 512 < 1 << 31
 
 
-def test_padding_outside_the_table_is_refused(voc):
+def test_padding_outside_the_table_is_refused(voc, monkeypatch):
+    monkeypatch.setattr(voc, "_numbers", lambda t, name: 0)  # the table need not be on a GPU to be refused
     w, t = torch.zeros((4, 3)), torch.zeros(4, dtype=torch.int64)
     for bad in (4, -5, 1 << 40):
         with pytest.raises(RuntimeError, match="padding_idx must be between -4 and 3"):
             voc.embed_tokens(w, t, padding_idx=bad)
-    assert voc._padding(None, 4) == (0, 0) and voc._padding(-4, 4) == (1, 0) and voc._padding(-1, 4) == (1, 3) and voc._padding(3, 4) == (1, 3)
+        with pytest.raises(RuntimeError, match="padding_idx must be between -4 and 3"):
+            voc.embed_tokens(w.clone().requires_grad_(True), t, padding_idx=bad)
+    given = lambda i: voc._padding(voc._optional_index(i, "padding_idx"), 4)
+    assert given(None) == (0, 0) and given(-4) == (1, 0) and given(-1) == (1, 3) and given(3) == (1, 3) and given(0) == (1, 0)
 
 
 @gpu
