@@ -181,6 +181,7 @@ class TokenLogprobsFunc(Function):
     def backward(ctx, g_logprob, g_entropy, g_top, _):
         if g_logprob is None and g_entropy is None and g_top is None:
             return None, None, None, None, None
+        _ops._no_tangents((g_logprob, g_entropy, g_top))
         logits, tokens, kept, ent, top_ix = ctx.saved_tensors
         V, dev = logits.shape[-1], logits.device
         inner, stride_outer, stride_inner = _logits_rows(logits)
@@ -297,6 +298,7 @@ class EmbedTokensFunc(Function):
     @staticmethod
     @_first_derivative
     def backward(ctx, grad_out):
+        _ops._no_tangents((grad_out,))
         (tokens,) = ctx.saved_tensors
         with _on(grad_out.device):
             d = grad_out.new_empty(ctx.shape)

@@ -1119,3 +1119,20 @@ def test_embedding_gradient_into_columns_of_a_wider_table(voc, dtype, into, n, V
         voc.embed_tokens_backward(g, t, part, scale=1.5, padding_idx=0)
         _close(part, want + start.double(), room + U * (want.abs() + start.double().abs()), into)
         assert bool((table[:, :first] == 7).all()) and bool((table[:, first + H:] == 7).all())
+
+
+@gpu
+def test_gradients_with_forward_mode_tangents_are_refused(voc):
+    """The derivative of a gradient along a direction in which the incoming gradient changes: the kernels would drop it."""
+    w = torch.randn((5, 3), device="cuda", requires_grad=True)
+    t = torch.tensor([0, 4, 4, 1], device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        for shape, call in (((4, 3), lambda: voc.embed_tokens(w, t)), ((4,), lambda: voc.token_logprobs(w[:4], t.clamp(max=2)).logprob),
+                            ((4, 2), lambda: voc.token_logprobs(w[:4], t.clamp(max=2), top=2).top_logprob),
+                            ((4,), lambda: voc.token_logprobs(w[:4], t.clamp(max=2), entropy=True).entropy)):
+            g = torch.randn(shape, device="cuda")
+            dual = torch.autograd.forward_ad.make_dual(g, torch.ones_like(g))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad([call()], [w], [dual])
+            d, = torch.autograd.grad([call()], [w], [g])  # without a tangent it goes on
+            assert bool(d.isfinite().all())
